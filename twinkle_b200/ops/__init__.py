@@ -816,6 +816,106 @@ def paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, scale: O
     return _open_gate(ref.paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, scale, window, softcap, sinks, chunk, terms), gate)
 
 
+class SharedPrefix(NamedTuple):
+    """Which sequences of a batch share the leading pages of their tables, cut into pieces of work for the kernel (``shared_prefix``)."""
+    plan: torch.Tensor        # int32: pieces, then a line per sequence
+    items: int
+    slots: int
+    sequences: int
+    heads: int
+    kv_heads: int
+    block_size: int
+
+
+def _prefix_items(sizes, blocks, block_size: int, group: int, kv_heads: int, sms: int):
+    """Pieces of work ``[first sequence, sequences, first block of 128 tokens, blocks of 128, tokens, slot]`` and per sequence ``[tokens, first slot, slots, row]``.
+
+    A tile of query rows holds ``128 // group`` sequences of one group.  Every SM runs one piece of one key head at a time; a piece costs its blocks and about two blocks'
+    time to begin and end.  Of all lengths of a piece the one is taken whose waves over the SMs cost least."""
+    tiles, at, per = [], 0, 128 // group
+    lines = [[0, 0, 0, 0] for _ in range(sum(sizes))]
+    for n, b in zip(sizes, blocks):
+        tokens, parts = b * block_size, (n + per - 1) // per
+        for i in range(parts if tokens else 0):      # a group's tiles are even
+            lo, hi = n * i // parts, n * (i + 1) // parts
+            tiles.append((at + lo, hi - lo, tokens, (tokens + 127) // 128))
+        at += n
+    if not tiles:
+        return [], lines
+    longest, most = max(t[3] for t in tiles), len(tiles) + 2 * sms // kv_heads
+    best = None
+    for cut in sorted({(longest + k - 1) // k for k in range(1, min(longest, most) + 1)}, reverse=True):
+        items = sum((t[3] + cut - 1) // cut for t in tiles)
+        if items > most:
+            break
+        cost = (items * kv_heads + sms - 1) // sms * (cut + 2)
+        if best is None or cost < best[0]:
+            best = (cost, cut)
+    items, slot = [], 0
+    for row, n, tokens, length in tiles:
+        parts = (length + best[1] - 1) // best[1]
+        for i in range(n):
+            lines[row + i] = [tokens, slot, parts, i * group]
+        for i in range(parts):
+            lo, hi = length * i // parts, length * (i + 1) // parts
+            items.append([row, n, lo, hi - lo, tokens, slot, 0, 0])
+            slot += 1
+    return items, lines
+
+
+def shared_prefix(sizes, blocks, block_size: int, heads: int, kv_heads: int, device='cuda', items: int = 0) -> SharedPrefix:
+    """The plan of a batch for ``paged_attention_shared``: group ``g`` is the next ``sizes[g]`` sequences, the first ``blocks[g]`` entries of whose table rows are the
+    same pages (0: nothing shared).  It holds for all layers and steps until a group changes; ``items``: pieces that it has room for at least, so that another plan
+    can be copied into a captured one (``prefix_items``)."""
+    sizes, blocks = [int(n) for n in sizes], [int(b) for b in blocks]
+    if len(sizes) != len(blocks) or any(n < 1 for n in sizes) or any(b < 0 for b in blocks) or block_size < 1:
+        raise ValueError('shared_prefix: a size of at least one sequence and a number of shared pages per group')
+    if kv_heads < 1 or heads % kv_heads or heads // kv_heads > 128:
+        raise ValueError(f'shared_prefix: {heads} query heads on {kv_heads} key heads')
+    work, lines = _prefix_items(sizes, blocks, block_size, heads // kv_heads, kv_heads, ext().num_sms() if torch.device(device).type == 'cuda' else 148)
+    room = max(len(work), items)
+    flat = [x for w in work for x in w] + [0] * (8 * (room - len(work))) + [x for l in lines for x in l]
+    return SharedPrefix(torch.tensor(flat, dtype=torch.int32).to(device), room, room, len(lines), heads, kv_heads, block_size)
+
+
+def prefix_items(sequences: int, kv_heads: int, device='cuda') -> int:
+    """Pieces that the plan of any ``sequences`` fits."""
+    return sequences + 2 * (ext().num_sms() if torch.device(device).type == 'cuda' else 148) // kv_heads
+
+
+def paged_attention_shared(q, k_cache, v_cache, block_tables, seq_lens, prefix: SharedPrefix, scale: Optional[float] = None):
+    """``paged_attention_decode`` for sequences that share pages: the shared ones are read once per group.  The table rows of a group begin with the same pages and
+    the first sequence of a group is a live one; a sequence shorter than what its group shares attends to its own length.  A page outside the pools counts as zeros and sets the error word.
+
+    bf16 caches of one width, 64 or 128, with pages of a multiple of 8 tokens; the rest goes through ``paged_attention_decode``, which reads all pages per sequence."""
+    if prefix.sequences != q.shape[0] or prefix.heads != q.shape[1] or prefix.kv_heads != k_cache.shape[2] or prefix.block_size != k_cache.shape[1]:
+        raise ValueError(f'paged_attention_shared: a plan for {prefix.sequences} sequences of {prefix.heads} / {prefix.kv_heads} heads and pages of {prefix.block_size}, got q '
+                         f'{tuple(q.shape)} and pools {tuple(k_cache.shape)}')
+    scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
+    if (_cuda(q) and prefix.items and q.shape[0] and q.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16 and k_cache.shape == v_cache.shape and q.shape[-1] in (64, 128)
+            and prefix.block_size % 8 == 0 and k_cache.is_contiguous() and v_cache.is_contiguous() and all(t.data_ptr() % 16 == 0 for t in (q, k_cache, v_cache))):
+        return ext().paged_attn_shared(q.contiguous(), k_cache, v_cache, block_tables.to(torch.int32).contiguous(), seq_lens.to(torch.int32).contiguous(), prefix.plan, prefix.items,
+                                       prefix.slots, scale)
+    return paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, scale)
+
+
+def cache_copy(pools, src, dst, tokens=None) -> None:
+    """In every pool ``[rows, ...]`` row ``dst[i]`` becomes row ``src[i]``, or with ``tokens`` its first ``tokens[i]`` entries along the second dimension do: pages of a paged
+    cache that fork or move, slots of recurrent state.  One launch for all pools and up to 2048 pairs.  The pairs are lists of numbers (they travel with the launch).  A row that is written is neither
+    written nor read by another pair."""
+    pools = [p for p in pools if p is not None]
+    if not pools:
+        return
+    src, dst, tokens = ([int(x) for x in v] for v in (src, dst, () if tokens is None else tokens))
+    if len(src) != len(dst) or (tokens and len(tokens) != len(src)):
+        raise ValueError('cache_copy: one destination (and number of tokens) per source')
+    if not src:
+        return
+    if all(_cuda(p) for p in pools):
+        return ext().cache_copy(pools, src, dst, tokens)
+    ref.cache_copy(pools, src, dst, tokens)
+
+
 def cache_write(k_pool, v_pool, rows, k, v) -> None:
     """Store ``k, v [T, heads, width]`` in rows ``rows [T]`` (block · block size + offset) of the paged pools ``[blocks, block size, heads, width]``.
     The kernel leaves out a row outside the pools and sets the error word, which ``NativeEngine.generate`` raises on."""
@@ -1000,6 +1100,121 @@ def fused_linear_logprob(hidden, weight, labels, temperature: float = 1.0, with_
         lp, ent = _FusedLinearLogprob.apply(hidden, weight, labels, temperature, with_entropy, chunk, wgrad_out)
         return lp, (ent if with_entropy else None)
     return ref.fused_linear_logprob(hidden, weight, labels, temperature, with_entropy)
+
+
+# ------------------------------------------------------------------ losses
+_POLICY = {'ratio': ('token', 'sequence'), 'surrogate': ('clip', 'soft', 'weight'), 'reduce': ('sequence', 'token', 'sum')}
+_PREFERENCE = ('sigmoid', 'hinge', 'ipo', 'kto_pair', 'simpo', 'orpo')
+
+
+def _loss_rows(what: str, logps, labels, per_token, per_row):
+    """Checks shapes; masks come as bool, labels as int64."""
+    if logps.dim() != 2 or labels.shape != logps.shape:
+        raise ValueError(f'{what}: log-probs {tuple(logps.shape)} and labels {tuple(labels.shape)}: both [rows, tokens]')
+    for name, t in per_token.items():
+        if t is not None and t.shape != logps.shape:
+            raise ValueError(f'{what}: {name} {tuple(t.shape)} for log-probs {tuple(logps.shape)}')
+    for name, t in per_row.items():
+        if t is not None and t.shape != logps.shape and t.shape != logps.shape[:1]:
+            raise ValueError(f'{what}: {name} {tuple(t.shape)} for log-probs {tuple(logps.shape)}: a number per row or per token')
+    return labels if labels.dtype in (torch.bool, torch.int64) else labels.long()
+
+
+def _side_by_side(t):
+    """fp32 with the tokens of a row side by side (rows may be anywhere), on the kernels' terms."""
+    if t is None:
+        return None
+    t = t if t.dtype in (torch.float32, torch.bool, torch.int64) else t.float()
+    return t if t.dim() == 1 or t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
+
+
+class _PolicyLoss(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, logps, entropies, labels, advantages, old, reference, args, entropy_coef, ignore_index):
+        loss, stats, deriv, weight = ext().policy_loss_fwd(logps, labels, advantages, old, reference, entropies, *args, ignore_index, ctx.needs_input_grad[0])
+        ctx.save_for_backward(deriv, weight, labels)
+        ctx.args = (entropy_coef, ignore_index)
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gloss, _gstats):
+        deriv, weight, labels = ctx.saved_tensors
+        need_lp, need_ent = ctx.needs_input_grad[:2]
+        grad, grad_ent = ext().policy_loss_bwd(gloss.float().contiguous(), deriv if need_lp else None, weight, labels, *ctx.args, need_ent)
+        return (grad if need_lp else None, grad_ent if need_ent else None) + (None, ) * 7
+
+
+def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entropies=None, ratio: str = 'token', surrogate: str = 'clip', reduce: str = 'sequence', epsilon: float = 0.2,
+                epsilon_high: Optional[float] = None, beta: float = 0.0, entropy_coef: float = 0.0, tau=(1.0, 1.0), denominator: float = 1.0, ignore_index: int = -100):
+    """``(loss, stats)`` of a policy step; differentiable by ``logps`` and ``entropies``.
+
+    ``logps [B, S]``; ``labels [B, S]``: tokens whose label is ``ignore_index`` (or a mask that is false) do not count; ``advantages`` per row ``[B]`` or per token; ``old_logps`` (the log-probs
+    themselves when left out), ``ref_logps`` (used when ``beta`` is positive) and ``entropies`` (used with ``entropy_coef``) ``[B, S]``.  With ``l = clamp(logp − old, ±20)``, its mean over the row
+    for ``ratio='sequence'``, and ``r = e^l`` a token costs ``−min(r A, clamp(r, 1 − epsilon, 1 + epsilon_high) A)`` (``clip``), ``−σ(τ (r − 1)) 4 A / τ`` with ``τ`` by the sign of A (``soft``) or
+    ``−min(r, 1 + epsilon) A logp`` with the weight held fixed (``weight``), plus ``beta (e^d − d − 1)`` with ``d = ref − logp``, minus ``entropy_coef`` times its entropy.  ``reduce``: mean over rows of
+    each row's mean, sum over the number of tokens, or sum over ``denominator``.  ``stats``: KL to the old policy, shares of tokens below and above the bounds, number of tokens."""
+    for name, value in (('ratio', ratio), ('surrogate', surrogate), ('reduce', reduce)):
+        if value not in _POLICY[name]:
+            raise ValueError(f'policy_loss: {name} is one of {_POLICY[name]}, not {value!r}')
+    epsilon_high = epsilon if epsilon_high is None else epsilon_high
+    if not 0 <= epsilon or not 0 <= epsilon_high or not denominator > 0 or not all(t > 0 for t in tau):
+        raise ValueError('policy_loss: bounds of zero or more, a positive denominator and positive temperatures')
+    if entropy_coef and entropies is None:
+        raise ValueError('policy_loss: entropy_coef needs entropies')
+    advantages = advantages[:, 0] if advantages.dim() == 2 and advantages.shape[1] == 1 != logps.shape[-1] else advantages
+    entropies, ref_logps = entropies if entropy_coef else None, ref_logps if beta > 0 else None
+    labels = _loss_rows('policy_loss', logps, labels, {'old_logps': old_logps, 'ref_logps': ref_logps, 'entropies': entropies}, {'advantages': advantages})
+    constants = [t for t in (advantages, old_logps, ref_logps) if t is not None]
+    if _cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not (torch.is_grad_enabled() and any(t.requires_grad for t in constants)):
+        args = (_POLICY['ratio'].index(ratio), _POLICY['surrogate'].index(surrogate), _POLICY['reduce'].index(reduce), float(epsilon), float(epsilon_high), float(beta), float(entropy_coef),
+                float(tau[0]), float(tau[1]), float(denominator))
+        return _PolicyLoss.apply(_side_by_side(logps), _side_by_side(entropies), _side_by_side(labels), *(_side_by_side(t) for t in (advantages, old_logps, ref_logps)), args,
+                                 float(entropy_coef), int(ignore_index))
+    return ref.policy_loss(logps, labels, advantages, old_logps, ref_logps, entropies, ratio, surrogate, reduce, epsilon, epsilon_high, beta, entropy_coef, tau, denominator, ignore_index)
+
+
+class _PreferenceLoss(torch.autograd.Function):
+
+    @staticmethod
+    def forward(ctx, logps, labels, reference, args, ignore_index):
+        loss, stats, coef = ext().preference_loss_fwd(logps, labels, reference, *args, ignore_index)
+        ctx.save_for_backward(coef, labels)
+        ctx.ignore_index = ignore_index
+        ctx.mark_non_differentiable(stats)
+        return loss, stats
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gloss, _gstats):
+        coef, labels = ctx.saved_tensors
+        return ext().preference_loss_bwd(gloss.float().contiguous(), coef, labels, ctx.ignore_index), None, None, None, None
+
+
+def preference_loss(logps, labels, ref_logps=None, form: str = 'sigmoid', beta: float = 0.1, gamma: float = 0.0, label_smoothing: float = 0.0, nll_weight: float = 0.0,
+                    ignore_index: int = -100):
+    """``(loss, stats)`` of pairs of rows, chosen ``0::2`` and rejected ``1::2``; differentiable by ``logps [B, S]``.
+
+    A row's level is the sum of its log-probs less that of ``ref_logps`` (``[B, S]``, or ``[B]`` summed already), for ``simpo`` and ``orpo`` their mean per token without a reference.  With
+    ``z = beta (chosen − rejected) − gamma`` a pair costs ``−log σ(z)``, smoothed (``sigmoid``, ``simpo``), ``max(0, 1 − z)`` (``hinge``), ``(z − 1 / (2 beta))²`` (``ipo``), ``1 − σ(beta chosen) + σ(beta rejected)``
+    (``kto_pair``) or ``−beta log σ`` of the log odds ratio (``orpo``); pairs are averaged, and ``nll_weight`` times the chosen rows' negative log-likelihood per chosen token is added.  ``stats``: ``beta`` times the
+    mean levels of the chosen and rejected rows and of their difference, share of pairs whose chosen row is above, mean summed log-probs of both."""
+    if form not in _PREFERENCE:
+        raise ValueError(f'preference_loss: form is one of {_PREFERENCE}, not {form!r}')
+    if form == 'ipo' and beta == 0:
+        raise ValueError('preference_loss: ipo divides by beta')
+    ref_logps = None if form in ('simpo', 'orpo') else ref_logps
+    labels = _loss_rows('preference_loss', logps, labels, {}, {'ref_logps': ref_logps})
+    if logps.shape[0] % 2:
+        raise ValueError(f'preference_loss: rows in pairs, got {logps.shape[0]}')
+    gamma, label_smoothing = (gamma if form in ('sigmoid', 'simpo', 'hinge', 'ipo') else 0.0), (label_smoothing if form in ('sigmoid', 'simpo') else 0.0)
+    if (_cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16)
+            and not (torch.is_grad_enabled() and ref_logps is not None and ref_logps.requires_grad)):
+        args = (_PREFERENCE.index(form), float(beta), float(gamma), float(label_smoothing), float(nll_weight))
+        return _PreferenceLoss.apply(_side_by_side(logps), _side_by_side(labels), _side_by_side(ref_logps), args, int(ignore_index))
+    return ref.preference_loss(logps, labels, ref_logps, form, beta, gamma, label_smoothing, nll_weight, ignore_index)
 
 
 # ------------------------------------------------------------------- adamw

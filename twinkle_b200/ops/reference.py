@@ -484,6 +484,88 @@ def attention_varlen(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     return (out, lse) if return_lse else out
 
 
+def cache_copy(pools, src, dst, tokens=()) -> None:
+    """Row ``dst[i]`` of every pool becomes row ``src[i]`` (its first ``tokens[i]`` entries)."""
+    rows = pools[0].shape[0]
+    if any(p.shape[0] != rows for p in pools) or any(not 0 <= r < rows for r in list(src) + list(dst)):
+        raise RuntimeError(f'cache_copy: rows outside pools of {rows}, or pools of unequal size')
+    if tokens and (any(p.dim() < 2 or p.shape[1] != pools[0].shape[1] for p in pools) or any(not 0 <= n <= pools[0].shape[1] for n in tokens)):
+        raise RuntimeError('cache_copy: tokens of a row of pools of one page size')
+    if len(set(dst)) != len(dst) or set(src) & set(dst):
+        raise RuntimeError('cache_copy: a row is written twice, or read and written')
+    for p in pools:
+        if not tokens:
+            p[list(dst)] = p[list(src)]
+            continue
+        for s, d, n in zip(src, dst, tokens):
+            p[d, :n] = p[s, :n]
+
+
+def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entropies=None, ratio='token', surrogate='clip', reduce='sequence', epsilon=0.2, epsilon_high=None, beta=0.0,
+                entropy_coef=0.0, tau=(1.0, 1.0), denominator=1.0, ignore_index=-100):
+    """See ``ops.policy_loss``; differentiable by everything."""
+    mask = labels if labels.dtype == torch.bool else labels != ignore_index
+    keep = lambda t: torch.where(mask, t, torch.zeros_like(t))  # noqa: E731   a NaN in a masked place stays there
+    n, total = mask.sum(-1, keepdim=True).clamp_min(1).to(logps.dtype), mask.sum().to(logps.dtype)
+    lp = keep(logps)
+    lr = torch.clamp(lp - (lp.detach() if old_logps is None else keep(old_logps.to(logps.dtype))), -20.0, 20.0)
+    if ratio == 'sequence':
+        lr = (lr.sum(-1, keepdim=True) / n).expand_as(lr)
+    r = torch.exp(lr)
+    adv = keep((advantages if advantages.dim() == 2 else advantages[:, None]).to(logps.dtype).expand_as(logps))
+    lo, hi = 1.0 - epsilon, 1.0 + (epsilon if epsilon_high is None else epsilon_high)
+    if surrogate == 'clip':
+        f = -torch.min(r * adv, torch.clamp(r, lo, hi) * adv)
+    elif surrogate == 'soft':
+        t = torch.where(adv > 0, torch.full_like(adv, tau[0]), torch.full_like(adv, tau[1]))
+        f = -torch.sigmoid(t * (r - 1.0)) * 4.0 / t * adv
+    else:
+        f = -torch.clamp(r, max=1.0 + epsilon).detach() * adv * lp
+    if ref_logps is not None and beta > 0:
+        d = keep(ref_logps.to(logps.dtype)) - lp
+        f = f + beta * (torch.exp(d) - d - 1.0)
+    if entropy_coef:
+        f = f - entropy_coef * keep(entropies.to(logps.dtype))
+    f = keep(f)
+    if reduce == 'sequence':
+        loss = (f.sum(-1, keepdim=True) / n).mean()
+    else:
+        loss = f.sum() / (total.clamp_min(1.0) if reduce == 'token' else denominator)
+    with torch.no_grad():
+        m = mask.to(logps.dtype)
+        stats = torch.stack([((r - 1.0 - lr) * m).sum(), ((r < lo) * m).sum(), ((r > hi) * m).sum(), total]) / torch.stack([total.clamp_min(1.0)] * 3 + [torch.ones_like(total)])
+    return loss, stats
+
+
+def preference_loss(logps, labels, ref_logps=None, form='sigmoid', beta=0.1, gamma=0.0, label_smoothing=0.0, nll_weight=0.0, ignore_index=-100):
+    """See ``ops.preference_loss``; differentiable by everything."""
+    mask = labels if labels.dtype == torch.bool else labels != ignore_index
+    total = lambda t: torch.where(mask, t, torch.zeros_like(t)).sum(-1)  # noqa: E731
+    seq, n = total(logps), mask.sum(-1)
+    if form in ('simpo', 'orpo'):
+        level = seq / n.clamp_min(1)
+    else:
+        level = seq if ref_logps is None else seq - (ref_logps.to(logps.dtype) if ref_logps.dim() == 1 else total(ref_logps.to(logps.dtype)))
+    c, r = level[0::2], level[1::2]
+    z = beta * (c - r) - gamma
+    if form in ('sigmoid', 'simpo'):
+        f = -F.logsigmoid(z) * (1 - label_smoothing) - F.logsigmoid(-z) * label_smoothing
+    elif form == 'hinge':
+        f = torch.relu(1 - z)
+    elif form == 'ipo':
+        f = (z - 1 / (2 * beta))**2
+    elif form == 'kto_pair':
+        f = 1 - torch.sigmoid(beta * c) + torch.sigmoid(beta * r)
+    else:
+        f = -beta * F.logsigmoid((c - r) - (torch.log1p(-torch.exp(c).clamp(max=1 - 1e-6)) - torch.log1p(-torch.exp(r).clamp(max=1 - 1e-6))))
+    loss = f.mean()
+    if nll_weight:
+        loss = loss - nll_weight * seq[0::2].sum() / n[0::2].sum().clamp_min(1)
+    with torch.no_grad():
+        stats = torch.stack([beta * c.mean(), beta * r.mean(), beta * (c - r).mean(), (c > r).to(logps.dtype).mean(), seq[0::2].mean(), seq[1::2].mean()])
+    return loss, stats
+
+
 def paged_attention_decode(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_tables: torch.Tensor,
                            seq_lens: torch.Tensor, scale: Optional[float] = None, window: Optional[int] = None,
                            softcap: Optional[float] = None, sinks: Optional[torch.Tensor] = None, chunk: int = 0, terms=None) -> torch.Tensor:
