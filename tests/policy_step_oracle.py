@@ -110,7 +110,7 @@ def preference(logps, labels, ref=None, form='sigmoid', beta=0.1, gamma=0.0, lab
     else:
         away = [0.0] * len(rows) if ref is None else [x if ref.dim() == 1 else torch.where(m, x, torch.zeros_like(x)).sum() for m, x in zip(mask, ref)]
         level = [r - a for r, a in zip(rows, away)]
-    log_sigmoid = lambda z: -torch.log1p(torch.exp(-z)) if float(z) > 0 else z - torch.log1p(torch.exp(z))  # noqa: E731
+    log_sigmoid = lambda z: -torch.log1p(torch.exp(-z)) if float(z.detach()) > 0 else z - torch.log1p(torch.exp(z))  # noqa: E731
     each = []
     for c, r in zip(level[0::2], level[1::2]):
         z = beta * (c - r) - gamma

@@ -430,3 +430,170 @@ def test_losses_keep_to_what_needs_a_gradient(E):
     half = x['logps'].bfloat16().requires_grad_()
     d = ops.policy_loss(half, x['labels'], x['adv'], x['old'])[0]
     assert torch.autograd.grad(d, half)[0].dtype == torch.bfloat16
+
+
+# ------------------------------------------------------------- used together
+def test_a_policy_step_end_to_end(E):
+    """A group is sampled from a shared prompt on captured steps, its answers are scored and trained on: one run of all four operators."""
+    from twinkle_b200 import ops
+    from twinkle_b200.data_format import SamplingParams
+    from twinkle_b200.loss import DPOLoss, GRPOLoss
+    from twinkle_b200.models import build_model, preset
+    from twinkle_b200.models.decoder import PackedBatch
+    from twinkle_b200.sampler.engine import NativeEngine
+    cfg = preset('qwen3-8b', num_hidden_layers=2, hidden_size=512, intermediate_size=1024, num_attention_heads=8, num_key_value_heads=2, vocab_size=1024)
+    model = build_model(cfg, device='cuda', dtype=torch.bfloat16, seed=0)
+    calls = {n: 0 for n in ('paged_attention_shared', 'cache_copy')}
+    real = {n: getattr(ops, n) for n in calls}
+    for n in calls:
+        def counted(*a, _n=n, **k):
+            calls[_n] += 1
+            return real[_n](*a, **k)
+        setattr(ops, n, counted)
+    try:
+        eng = NativeEngine(model, cfg, num_blocks=200, block_size=16, share_prompts=True)
+        prompts = [[(7 * i + 3) % 900 for i in range(300)], [(3 * i + 1) % 900 for i in range(64)]]
+        res = eng.generate(prompts, [SamplingParams(max_tokens=20, temperature=1.0, num_samples=4) for _ in prompts])
+    finally:
+        for n, f in real.items():
+            setattr(ops, n, f)
+    assert calls['cache_copy'] == 1 and calls['paged_attention_shared'] > 0 and any(k[2] for k in eng._graphs)
+    # the log-prob of every sampled token, from a forward over the whole answer
+    rows = [(p, s) for p, r in zip(prompts, res) for s in r.sequences]
+    assert len(rows) == 8 and sorted(eng.cache.free) == list(range(1, 200))
+    S = max(len(p) + len(s.tokens) for p, s in rows)
+    labels, logps, old = torch.full((8, S), -100), [], torch.zeros(8, S)
+    hidden = []
+    for b, (p, s) in enumerate(rows):
+        toks, n = p + s.tokens, len(p)
+        batch_ = PackedBatch(torch.tensor(toks, device='cuda'), torch.arange(len(toks), device='cuda'), torch.tensor([0, len(toks)], dtype=torch.int32, device='cuda'), len(toks))
+        with torch.no_grad():
+            hidden.append(model(batch_))
+        labels[b, n - 1:len(toks) - 1] = torch.tensor(s.tokens)
+        old[b, n - 1:len(toks) - 1] = torch.tensor(s.logprobs)
+    x = torch.zeros(8, S, 512, dtype=torch.bfloat16, device='cuda')
+    for b, h in enumerate(hidden):
+        x[b, :h.shape[0]] = h
+    x.requires_grad_()
+    flat = labels.clamp_min(0).reshape(-1).cuda()
+    logps = ops.fused_linear_logprob(x.reshape(8 * S, 512), model.head_weight().detach(), flat)[0].view(8, S)
+    mask = labels != -100
+    assert (logps.detach().cpu() - old)[mask].abs().max() < 0.05          # bf16 activations of two routes through the model
+    losses = [GRPOLoss(epsilon=0.2, beta=0.04)({'labels': labels}, {'logps': logps}, old_logps=old, ref_logps=old, advantages=[1.0, -1.0, 0.5, -0.5] * 2)['loss'],
+              DPOLoss(beta=0.1)({'labels': labels}, {'logps': logps}, ref_logps=old)['loss']]
+    for loss in losses:
+        g, = torch.autograd.grad(loss, x, retain_graph=True)
+        assert torch.isfinite(g).all() and g[mask.cuda()].abs().sum() > 0 and not g[~mask.cuda()].any()
+
+
+@pytest.mark.parametrize('stack', ['tiny-dense', 'tiny-hybrid', 'tiny-deepseek', 'pomelix', 'moronex', 'puzonex'])
+def test_groups_share_their_prompt(E, stack, tmp_path):
+    """Greedy answers of a group in fp32 are those of separate sequences; in bf16 a captured and an eager step agree."""
+    from tests.test_policy_step import _engine, run_group
+    runs = [run_group(_engine(stack, tmp_path, ('cuda', 'float32'), share=s)) for s in (False, True)]
+    for a, b in zip(*runs):
+        for x, y in zip(a.sequences, b.sequences):
+            assert x.tokens == y.tokens and x.logprobs == pytest.approx(y.logprobs, abs=1e-3)
+    got = []
+    for graphs in (True, False):
+        e = _engine(stack, tmp_path, ('cuda', 'bfloat16'), share=True)
+        e.use_cuda_graphs = graphs
+        got.append(run_group(e))
+        assert sorted(e.cache.free) == list(range(1, e.cache.num_blocks)) and not e.cache.sharers
+    for a, b in zip(*got):
+        for x, y in zip(a.sequences, b.sequences):
+            assert x.tokens == y.tokens and x.logprobs == pytest.approx(y.logprobs, abs=1e-3)
+
+
+def test_a_group_that_shrinks_and_is_compacted(E):
+    """Steps of a group on captured graphs, with fewer members from step to step and the cache compacted in between, against separate sequences."""
+    from twinkle_b200.data_format import SamplingParams
+    from twinkle_b200.models import build_model, preset
+    from twinkle_b200.sampler.engine import NativeEngine, _Seq
+    cfg = preset('qwen3-8b', num_hidden_layers=2, hidden_size=512, intermediate_size=1024, num_attention_heads=8, num_key_value_heads=2, vocab_size=1024)
+    model = build_model(cfg, device='cuda', dtype=torch.bfloat16, seed=0)
+    prompt = [(7 * i + 3) % 900 for i in range(211)]
+    steps = {}
+    for share in (False, True):
+        eng = NativeEngine(model, cfg, num_blocks=160, block_size=16, max_batch=8, share_prompts=share)
+        seqs = [_Seq(0, list(prompt), SamplingParams(max_tokens=8)) for _ in range(6)] + [_Seq(1, prompt[:40], SamplingParams(max_tokens=8))]
+        if share:
+            eng.prefill([seqs[0], seqs[6]])
+            eng.fork(seqs[0], seqs[1:6])
+        else:
+            eng.prefill(seqs)
+        steps[share] = []
+        for n in range(5):
+            for i, s in enumerate(seqs):
+                s.tokens.append((37 * n + s.request + 11 * len(seqs)) % 900)
+            steps[share].append(eng.decode_step(seqs, torch.tensor([s.tokens[-1] for s in seqs], device='cuda')).clone())
+            if n in (1, 2):
+                eng.release([seqs.pop(0)])
+            if n == 2:
+                eng.compact(seqs, 100)
+    for a, b in zip(steps[False], steps[True]):
+        assert (a - b).norm() / a.norm() < 2e-2
+    assert E.read_and_clear_error() == 0
+
+
+@pytest.mark.parametrize('name,kwargs', [('GRPOLoss', dict(epsilon=0.2, epsilon_high=0.3, beta=0.05)), ('GRPOLoss', dict(entropy_coef=0.01)), ('GSPOLoss', dict(epsilon=0.01)),
+                                         ('SAPOLoss', dict(tau_neg=1.5)), ('CISPOLoss', dict(epsilon=0.1)), ('BNPOLoss', {}), ('DRGRPOLoss', dict(max_completion_length=64))])
+@pytest.mark.parametrize('form', ['rows', 'list', 'ragged', 'tokens', 'one'])
+def test_policy_loss_classes(E, name, kwargs, form):
+    """The classes on the GPU against their methods on the CPU, however the advantages come."""
+    from twinkle_b200 import loss as L
+    x = _policy_inputs(6, 80, 12)
+    labels = x['labels'].cpu()
+    adv = {'rows': x['adv'][:, 0], 'list': x['adv'][:, 0].tolist(), 'ragged': [r[m].tolist() for r, m in zip(x['adv'].cpu(), labels != -100)], 'tokens': x['adv'], 'one': 0.7}[form]
+    if form == 'ragged':
+        adv = [r or [0.0] for r in adv]
+    got = []
+    for device in ('cuda', 'cpu'):
+        lp = x['logps'].detach().to(device).requires_grad_()
+        before = E.launch_count()
+        out = getattr(L, name)(**kwargs)({'labels': labels}, {'logps': lp, 'entropies': x['ent'].to(device)}, old_logps=x['old'].to(device), ref_logps=x['ref'].to(device), advantages=adv)['loss']
+        assert (E.launch_count() > before) == (device == 'cuda')
+        got.append((out.detach().cpu(), torch.autograd.grad(out, lp)[0].cpu()))
+    (a, ga), (b, gb) = got
+    # the methods work in fp32 throughout: 480 terms of up to 2^3 of either sign
+    assert abs(float(a - b)) <= 2**-17 * max(1.0, abs(float(b))) and (ga - gb).abs().max() <= 2**-17 * gb.abs().max()
+
+
+def test_policy_losses_of_other_rules_keep_their_methods(E):
+    from twinkle_b200.loss import GRPOLoss
+
+    class Mine(GRPOLoss):
+        def _surrogate(self, ratio, adv, logps):
+            return -ratio * adv * 3.0
+
+    x = _policy_inputs(4, 20, 13)
+    before = E.launch_count()
+    got = Mine()({'labels': x['labels']}, {'logps': x['logps']}, old_logps=x['logps'], advantages=[1.0] * 4)['loss']
+    assert E.launch_count() == before and abs(float(got) + 3.0 * float(((x['labels'] != -100).any(-1)).float().mean())) < 1e-5
+
+
+@pytest.mark.parametrize('name,kwargs', [('DPOLoss', dict(loss_type=t)) for t in ('sigmoid', 'hinge', 'ipo', 'kto_pair')] +
+                         [('DPOLoss', dict(label_smoothing=0.1, sft_weight=0.3)), ('DPOLoss', dict(reference_free=True)), ('SimPOLoss', {}), ('CPOLoss', {}), ('ORPOLoss', {})])
+@pytest.mark.parametrize('form', ['tokens', 'short', 'long', 'rows', 'pairs'])
+def test_preference_loss_classes(E, name, kwargs, form):
+    from twinkle_b200 import loss as L
+    x = _policy_inputs(6, 40, 14)
+    x['labels'][3, 1] = 5                     # no row without an answer
+    labels, ref = x['labels'].cpu(), x['ref'].cpu()
+    seq = torch.where(labels != -100, ref, torch.zeros_like(ref)).sum(-1)
+    extra = {'tokens': dict(ref_logps=ref), 'short': dict(ref_outputs={'logps': ref[:, :30]}), 'long': dict(ref_logps=torch.cat([ref, ref], 1)), 'rows': dict(ref_logps=seq),
+             'pairs': dict(ref_chosen_logps=seq[0::2], ref_rejected_logps=seq[1::2])}[form]
+    if kwargs.get('reference_free') and form == 'tokens':
+        extra = {}
+    got, stats = [], []
+    for device in ('cuda', 'cpu'):
+        lp = x['logps'].detach().to(device).requires_grad_()
+        before = E.launch_count()
+        obj = getattr(L, name)(**kwargs)
+        out = obj({'labels': labels}, {'logps': lp}, **extra)['loss']
+        assert (E.launch_count() > before) == (device == 'cuda')
+        got.append((out.detach().cpu(), torch.autograd.grad(out, lp)[0].cpu()))
+        stats.append(getattr(obj, 'last_stats', {}))
+    (a, ga), (b, gb) = got
+    assert abs(float(a - b)) <= 2**-16 * max(1.0, abs(float(b))) and (ga - gb).abs().max() <= 2**-15 * gb.abs().max()
+    assert stats[0].keys() == stats[1].keys() and all(stats[0][k] == pytest.approx(stats[1][k], rel=1e-4, abs=1e-4) for k in stats[0])

@@ -4,6 +4,8 @@ Parity: reference ``src/twinkle/loss/dpo.py:20-569`` — DPO with sigmoid /
 hinge / ipo / kto_pair forms, label smoothing, ``sft_weight``,
 ``reference_free``; SimPO, CPO, ORPO.  Rows ``0::2`` are chosen and ``1::2``
 rejected, so a contiguous data-parallel slice of even length keeps pairs whole.
+On a GPU fp32 log-probs go through ``ops.preference_loss``; classes derived from
+these keep to the PyTorch forms.
 """
 from __future__ import annotations
 
@@ -12,6 +14,7 @@ from typing import Any, Dict, Optional
 import torch
 import torch.nn.functional as F
 
+from .. import ops
 from ..data_format import LossOutput
 from .base import Loss, as_2d_labels, token_logps
 
@@ -29,6 +32,17 @@ class PreferenceLoss(Loss):
             raise AssertionError('preference batches interleave chosen/rejected rows; got an odd number of rows')
         seq = (logps * mask).sum(-1)
         return logps, mask, seq
+
+    def _rows(self, inputs, outputs):
+        """Labels and log-probs where the kernel takes them, else None."""
+        labels = as_2d_labels(inputs)
+        logps = outputs.get('logps')
+        if logps is not None and logps.dim() == 1:
+            logps = logps.unsqueeze(0)
+        if (type(self) not in _ON_KERNEL or logps is None or not logps.is_cuda or logps.dtype != torch.float32 or logps.shape != labels.shape or logps.numel() == 0
+                or logps.shape[0] % 2):
+            return None
+        return labels.to(logps.device), logps
 
     @staticmethod
     def _nll(chosen_seq_logps: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
@@ -71,6 +85,9 @@ class DPOLoss(PreferenceLoss):
         """The reference policy comes as ``ref_outputs`` / ``ref_logps`` (per token or per sequence, rows interleaved
         like the batch) or as the two sequence-level vectors ``ref_chosen_logps`` / ``ref_rejected_logps``
         (reference ``src/twinkle/loss/dpo.py:257-320``)."""
+        rows = self._rows(inputs, outputs)
+        if rows is not None:
+            return self._kernel_loss(*rows, ref_outputs if ref_outputs is not None else ref_logps, ref_chosen_logps, ref_rejected_logps)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         pc, pr = seq[0::2], seq[1::2]
         ref = None
@@ -109,6 +126,28 @@ class DPOLoss(PreferenceLoss):
         return LossOutput(loss=loss, num_tokens=0)
 
 
+    def _kernel_loss(self, labels, logps, ref, ref_chosen, ref_rejected) -> LossOutput:
+        if ref_chosen is not None and ref_rejected is not None:
+            rc, rr = (torch.as_tensor(r).to(logps.device, logps.dtype).reshape(-1) for r in (ref_chosen, ref_rejected))
+            pairs = logps.shape[0] // 2
+            if rc.numel() != pairs or rr.numel() != pairs:
+                raise ValueError(f'ref_chosen_logps / ref_rejected_logps must hold one value per pair ({pairs}), got {rc.numel()} / {rr.numel()}')
+            ref = torch.stack([rc, rr], -1).reshape(-1)
+        else:
+            if isinstance(ref, dict):
+                ref = ref.get('logps')
+            if ref is not None:
+                ref = (ref if torch.is_tensor(ref) else torch.as_tensor(ref)).to(logps.device, logps.dtype)
+                if ref.dim() == 2 and ref.shape[1] != logps.shape[1]:      # shorter rows end in nothing, longer ones are cut
+                    ref = F.pad(ref, (0, logps.shape[1] - ref.shape[1]))
+            elif not self.reference_free:
+                return LossOutput(loss=logps.sum() * 0.0, num_tokens=0)
+        loss, stats = ops.preference_loss(logps, labels, ref, self.loss_type, self.beta, label_smoothing=self.label_smoothing, nll_weight=max(self.sft_weight, 0.0),
+                                          ignore_index=self.ignore_index)
+        self.last_stats = dict(zip(('rewards/chosen', 'rewards/rejected', 'rewards/margins', 'rewards/accuracies', 'logps/chosen', 'logps/rejected'), stats.tolist()))
+        return LossOutput(loss=loss, num_tokens=0)
+
+
 class SimPOLoss(PreferenceLoss):
     """Length-normalised, reference-free: ``−logσ(β(avg_c − avg_r) − γ)``."""
 
@@ -117,6 +156,9 @@ class SimPOLoss(PreferenceLoss):
         self.beta, self.gamma = beta, gamma
 
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
+        rows = self._rows(inputs, outputs)
+        if rows is not None:
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='simpo', beta=self.beta, gamma=self.gamma, ignore_index=self.ignore_index)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         avg = seq / mask.sum(-1).clamp_min(1)
         z = self.beta * (avg[0::2] - avg[1::2]) - self.gamma
@@ -131,6 +173,9 @@ class CPOLoss(PreferenceLoss):
         self.beta, self.bc_coef = beta, bc_coef
 
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
+        rows = self._rows(inputs, outputs)
+        if rows is not None:
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], beta=self.beta, nll_weight=self.bc_coef, ignore_index=self.ignore_index)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         pref = -F.logsigmoid(self.beta * (seq[0::2] - seq[1::2])).mean()
         return LossOutput(loss=pref + self.bc_coef * self._nll(seq[0::2], mask), num_tokens=0)
@@ -144,9 +189,15 @@ class ORPOLoss(PreferenceLoss):
         self.lambda_orpo = lambda_orpo
 
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
+        rows = self._rows(inputs, outputs)
+        if rows is not None:
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='orpo', beta=self.lambda_orpo, nll_weight=1.0, ignore_index=self.ignore_index)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         avg = seq / mask.sum(-1).clamp_min(1)
         c, r = avg[0::2], avg[1::2]
         log_odds = (c - r) - (torch.log1p(-torch.exp(c).clamp(max=1 - 1e-6)) - torch.log1p(-torch.exp(r).clamp(max=1 - 1e-6)))
         loss = self._nll(seq[0::2], mask) - self.lambda_orpo * F.logsigmoid(log_odds).mean()
         return LossOutput(loss=loss, num_tokens=0)
+
+
+_ON_KERNEL = (DPOLoss, SimPOLoss, CPOLoss, ORPOLoss)

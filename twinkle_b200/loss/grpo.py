@@ -3,7 +3,9 @@
 Parity: reference ``src/twinkle/loss/grpo.py:13-437`` — GRPO plus the GSPO,
 SAPO, CISPO, BNPO and DR-GRPO variants, including the alignment rules for
 ragged ``old_logps`` / ``ref_logps`` / ``advantages``.  Each variant here is a
-(ratio rule, surrogate rule, aggregation rule) triple on one class.
+(ratio rule, surrogate rule, aggregation rule) triple on one class.  On a GPU the
+triple is computed by ``ops.policy_loss``; classes derived from these, whose rules
+may be others, and log-probs in other types than fp32 go through the methods.
 """
 from __future__ import annotations
 
@@ -12,6 +14,7 @@ from typing import Any, Dict, List, Optional, Sequence, Union
 import numpy as np
 import torch
 
+from .. import ops
 from ..data_format import LossOutput
 from .base import Loss, as_2d_labels, token_logps
 
@@ -56,7 +59,23 @@ def align_to_mask(values, mask: torch.Tensor, dtype=torch.float32) -> torch.Tens
     return out
 
 
+def row_values(values, B: int, device) -> Optional[torch.Tensor]:
+    """``values`` as one number per row ``[B]``, as ``align_to_mask`` would spread them; None where they are anything else."""
+    if isinstance(values, (int, float)):
+        values = [float(values)] * B
+    if isinstance(values, np.ndarray):
+        values = torch.from_numpy(values)
+    if torch.is_tensor(values):
+        if values.dim() > 1 or values.numel() not in (1, B):
+            return None
+        return values.detach().reshape(-1).to(device=device, dtype=torch.float32).expand(B)
+    if len(values) == B and all(isinstance(v, (int, float)) for v in values):
+        return torch.tensor([float(v) for v in values], dtype=torch.float32, device=device)
+    return None
+
+
 class GRPOLoss(Loss):
+    rules: Dict[str, str] = dict(ratio='token', surrogate='clip', reduce='sequence')     # of ``ops.policy_loss``; a class has its own
 
     def __init__(self, epsilon: float = 0.2, epsilon_high: Optional[float] = None, beta: float = 0.0,
                  entropy_coef: float = 0.0, ignore_index: int = -100, **kwargs):
@@ -88,6 +107,8 @@ class GRPOLoss(Loss):
         mask = (labels != self.ignore_index).to(logps.device)
         if advantages is None:
             return LossOutput(loss=logps.sum() * 0.0, num_tokens=0)
+        if self._on_kernel(labels, logps, outputs):
+            return LossOutput(loss=self._kernel_loss(labels.to(logps.device), logps, mask, outputs, old_logps, ref_logps, advantages, kwargs), num_tokens=0)
         old = logps.detach() if old_logps is None else align_to_mask(old_logps, mask, logps.dtype)
         adv = align_to_mask(advantages, mask, logps.dtype)
         ratio = torch.exp(self._log_ratio(logps, old, mask))
@@ -101,6 +122,27 @@ class GRPOLoss(Loss):
                 raise AssertionError("entropy_coef > 0 needs outputs['entropies']")
             per_token = per_token - self.entropy_coef * ent.to(per_token.dtype)
         return LossOutput(loss=self._aggregate(per_token, mask, **kwargs), num_tokens=0)
+
+    # on the kernel ---------------------------------------------------------
+    def _on_kernel(self, labels, logps, outputs) -> bool:
+        ent = outputs.get('entropies')
+        return ('rules' in type(self).__dict__ and logps.is_cuda and logps.dtype == torch.float32 and logps.dim() == 2 and logps.shape == labels.shape and logps.numel() > 0
+                and self.epsilon >= 0 and self.epsilon_high >= 0 and (self.entropy_coef <= 0.0 or (ent is not None and ent.shape == logps.shape)))
+
+    def _kernel_loss(self, labels, logps, mask, outputs, old_logps, ref_logps, advantages, kwargs) -> torch.Tensor:
+        grid = lambda v: None if v is None else align_to_mask(v, mask, logps.dtype)  # noqa: E731
+        adv = row_values(advantages, logps.shape[0], logps.device)
+        entropy_coef = max(self.entropy_coef, 0.0)
+        loss, stats = ops.policy_loss(logps, labels, grid(advantages) if adv is None else adv, grid(old_logps), grid(ref_logps) if self.beta > 0.0 else None,
+                                      outputs['entropies'] if entropy_coef else None, epsilon=self.epsilon, epsilon_high=self.epsilon_high, beta=self.beta, entropy_coef=entropy_coef,
+                                      ignore_index=self.ignore_index, **self.rules, **self._kernel_args(logps))
+        return self._kernel_reduced(loss, stats, kwargs)
+
+    def _kernel_args(self, logps) -> Dict[str, Any]:
+        return {}
+
+    def _kernel_reduced(self, loss: torch.Tensor, stats: torch.Tensor, kwargs) -> torch.Tensor:
+        return loss
 
     # metrics helpers -----------------------------------------------------
     @torch.no_grad()
@@ -117,6 +159,7 @@ class GRPOLoss(Loss):
 
 class GSPOLoss(GRPOLoss):
     """Sequence-level ratio: masked mean of the token log ratios, broadcast."""
+    rules = dict(ratio='sequence', surrogate='clip', reduce='sequence')
 
     def _log_ratio(self, logps, old_logps, mask):
         m = mask.to(logps.dtype)
@@ -128,6 +171,7 @@ class GSPOLoss(GRPOLoss):
 
 class SAPOLoss(GRPOLoss):
     """Soft gate ``σ(τ(r−1))·4/τ`` with a temperature chosen by the sign of A."""
+    rules = dict(ratio='token', surrogate='soft', reduce='sequence')
 
     def __init__(self, tau_pos: float = 1.0, tau_neg: float = 1.0, **kw):
         super().__init__(**kw)
@@ -138,8 +182,12 @@ class SAPOLoss(GRPOLoss):
         gate = torch.sigmoid(tau * (ratio - 1.0)) * 4.0 / tau
         return -gate * adv
 
+    def _kernel_args(self, logps):
+        return dict(tau=(self.tau_pos, self.tau_neg))
+
 
 class CISPOLoss(GRPOLoss):
+    rules = dict(ratio='token', surrogate='weight', reduce='sum')
 
     def _surrogate(self, ratio, adv, logps):
         return -torch.clamp(ratio, max=1.0 + self.epsilon).detach() * adv * logps  # reference loss/grpo.py:379
@@ -149,14 +197,20 @@ class CISPOLoss(GRPOLoss):
         n = mask.sum() if n is None else n
         return (per_token * mask).sum() / n
 
+    def _kernel_reduced(self, loss, stats, kwargs):
+        n = kwargs.get('num_items_in_batch')
+        return loss / (stats[3] if n is None else n)
+
 
 class BNPOLoss(GRPOLoss):
+    rules = dict(ratio='token', surrogate='clip', reduce='token')
 
     def _aggregate(self, per_token, mask, **kwargs):
         return (per_token * mask).sum() / mask.sum().clamp_min(1.0)
 
 
 class DRGRPOLoss(GRPOLoss):
+    rules = dict(ratio='token', surrogate='clip', reduce='sum')
 
     def __init__(self, max_completion_length: int = 1024, **kw):
         super().__init__(**kw)
@@ -164,3 +218,6 @@ class DRGRPOLoss(GRPOLoss):
 
     def _aggregate(self, per_token, mask, **kwargs):
         return (per_token * mask).sum() / (mask.shape[0] * self.max_completion_length)
+
+    def _kernel_args(self, logps):
+        return dict(denominator=float(logps.shape[0] * self.max_completion_length))

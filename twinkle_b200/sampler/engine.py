@@ -48,6 +48,7 @@ class PagedKVCache:
         self.conv = [mk(self.num_slots, *c) if c else None for c in self.cfg.conv_layout() or none]
         self.state = [torch.zeros(self.num_slots, *c, device=self.device) if c else None for c in self.cfg.state_layout() or none]
         self.free: List[int] = list(range(self.num_blocks - 1, 0, -1))
+        self.sharers: Dict[int, int] = {}          # blocks with several owners → owners beyond the first
         self.free_slots: List[int] = list(range(self.num_slots - 1, 0, -1))
 
     def drop(self) -> None:
@@ -79,7 +80,66 @@ class PagedKVCache:
         return [self.free.pop() for _ in range(n)]
 
     def release(self, blocks: Sequence[int]) -> None:
+        """Give an owner's blocks back; one with other owners stays theirs."""
+        if self.sharers:
+            mine, blocks = blocks, []
+            for b in mine:
+                left = self.sharers.get(b, 0)
+                if left > 1:
+                    self.sharers[b] = left - 1
+                elif left:
+                    del self.sharers[b]
+                else:
+                    blocks.append(b)
         self.free.extend(reversed(list(blocks)))
+
+    def fork(self, blocks: Sequence[int], n_tokens: int, n_blocks: Sequence[int]) -> Tuple[List[List[int]], List[Tuple[int, int, int]]]:
+        """Block lists of ``n_blocks[i]`` blocks each for continuations of a sequence whose first ``n_tokens`` tokens lie in ``blocks``: they
+        share its full blocks and own the rest.  Beside them the copies ``(from, to, tokens)`` that put the tokens of the last, partly filled block where each
+        continues it (``copy``)."""
+        full, rest = divmod(n_tokens, self.block_size)
+        own = self.allocate(sum(max(n, full + (rest > 0)) - full for n in n_blocks))
+        lists, copies, at = [], [], 0
+        for n in n_blocks:
+            mine = own[at:at + max(n, full + (rest > 0)) - full]
+            at += len(mine)
+            lists.append(list(blocks[:full]) + mine)
+            if rest:
+                copies.append((blocks[full], mine[0], rest))
+        for b in blocks[:full]:
+            self.sharers[b] = self.sharers.get(b, 0) + len(n_blocks)
+        return lists, copies
+
+    def copy(self, copies: Sequence[Tuple[int, int, int]], slots: Sequence[Tuple[int, int]] = ()) -> None:
+        """Tokens of blocks ``(from, to, tokens)`` in all layers' pools, and rows ``(from, to)`` of the history and state pools."""
+        if copies:
+            ops.cache_copy(self.k + self.v, *zip(*copies))
+        if slots and self.num_slots:
+            ops.cache_copy(self.conv + self.state, *zip(*slots))
+
+    def compact(self, lists: Sequence[List[int]], num_blocks: Optional[int] = None) -> None:
+        """Move the blocks of all live sequences, whose lists are given and renumbered in place, to the front of the pools; with ``num_blocks`` the pools are
+        then replaced by ones of that many blocks."""
+        live = {b for blocks in lists for b in blocks}
+        if len(live) + len(self.free) != self.num_blocks - 1 or live & set(self.free):
+            raise RuntimeError(f'{self.num_blocks - 1 - len(self.free)} blocks are in use, the lists name {len(live)}')
+        if num_blocks is not None and num_blocks <= len(live):
+            raise RuntimeError(f'{len(live)} live blocks do not fit a cache of {num_blocks}')
+        holes = [b for b in range(1, len(live) + 1) if b not in live]
+        place = dict(zip(sorted((b for b in live if b > len(live)), reverse=True), holes))
+        self.copy([(b, to, self.block_size) for b, to in place.items()])
+        for blocks in lists:
+            blocks[:] = [place.get(b, b) for b in blocks]
+        self.sharers = {place.get(b, b): n for b, n in self.sharers.items()}
+        if num_blocks is not None and num_blocks != self.num_blocks:
+            kept = len(live) + 1
+            for pools in (self.k, self.v):
+                for i, old in enumerate(pools):
+                    if old is not None:
+                        pools[i] = torch.zeros((num_blocks, ) + old.shape[1:], device=old.device, dtype=old.dtype)
+                        pools[i][:kept] = old[:kept]
+            self.num_blocks = num_blocks
+        self.free = list(range(self.num_blocks - 1, len(live), -1))
 
     def blocks_for(self, n_tokens: int) -> int:
         return (n_tokens + self.block_size - 1) // self.block_size
@@ -107,6 +167,7 @@ class _Seq:
     vision: Optional[Dict[str, Any]] = None   # pixel_values, image_grid_thw, mrope_position_ids [3, L] of a prompt with images
     rope_delta: int = 0                        # rotary position − token index for the tokens after the prompt (images compress positions)
     linear: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = field(default_factory=dict)  # layer → (conv rows, recurrent state) of linear-attention layers
+    origin: Optional['_Seq'] = None            # the sequence whose prompt this one shares (itself: others share its own)
 
     @property
     def length(self) -> int:
@@ -116,8 +177,11 @@ class _Seq:
 class NativeEngine:
 
     def __init__(self, model: DecoderModel, cfg: DecoderConfig, device=None, num_blocks: Optional[int] = None, block_size: int = 16,
-                 max_batch: int = 256, gpu_memory_utilization: float = 0.85, decode: Optional[Callable[[List[int]], str]] = None):
-        self.model, self.cfg = model, cfg
+                 max_batch: int = 256, gpu_memory_utilization: float = 0.85, decode: Optional[Callable[[List[int]], str]] = None, share_prompts: bool = False):
+        """``share_prompts``: sequences with the same prompt (the samples of a request, repeated prompts) run through it once, share its full cache
+        blocks and read them once per step.  Results then differ by the rounding of other tile shapes and orders of sums."""
+        self.model, self.cfg, self.share_prompts = model, cfg, share_prompts
+        self._plan: Tuple[Any, Optional[ops.SharedPrefix]] = (None, None)      # of the last step with shared prompts
         self.device = device or next(model.parameters()).device
         self.dtype = next(model.parameters()).dtype
         if num_blocks is None:
@@ -153,6 +217,50 @@ class NativeEngine:
             s.blocks = self.cache.allocate(self.cache.blocks_for(len(s.prompt) + (s.params.max_tokens or 0) + 1))
             s.state_slot = self.cache.allocate_slot()
 
+    def fork(self, origin: _Seq, seqs: Sequence[_Seq]) -> None:
+        """Let ``seqs`` continue the prompt of ``origin``, which has run: its full blocks are shared, the rest and the state are copied."""
+        lists, copies = self.cache.fork(origin.blocks, len(origin.prompt), [self.cache.blocks_for(len(s.prompt) + (s.params.max_tokens or 0) + 1) for s in seqs])
+        slots = []
+        for s, blocks in zip(seqs, lists):
+            s.blocks, s.state_slot, s.origin = blocks, self.cache.allocate_slot(), origin
+            s.linear, s.rope_delta, s.routed = dict(origin.linear), origin.rope_delta, None if origin.routed is None else list(origin.routed)
+            if s.state_slot:
+                slots.append((origin.state_slot, s.state_slot))
+        origin.origin = origin
+        self.cache.copy(copies, slots)
+
+    def compact(self, seqs: Sequence[_Seq], num_blocks: Optional[int] = None) -> None:
+        """Bring the blocks of all live sequences together at the front of the cache; with ``num_blocks`` the cache is given that size."""
+        self.cache.compact([s.blocks for s in seqs], num_blocks)
+        if num_blocks is not None:
+            self._graphs.clear()          # captured steps hold the addresses of the pools
+
+    def _shared(self, seqs: Sequence[_Seq], rows: int, captured: bool = False) -> Optional[ops.SharedPrefix]:
+        """The plan of a step whose sequences share prompts (None: nothing to share), filled up to ``rows`` sequences; ``captured``: with room for any plan of
+        that many."""
+        if not self.share_prompts or self.cfg.layer_specs is not None or not any(s.origin is not None for s in seqs):
+            return None
+        sizes, blocks, last = [], [], None
+        for s in seqs:
+            if s.origin is not None and s.origin is last:
+                sizes[-1] += 1
+            else:
+                sizes.append(1)
+                blocks.append(len(s.prompt) // self.cache.block_size if s.origin is not None else 0)
+            last = s.origin
+        blocks = [b if n > 1 else 0 for n, b in zip(sizes, blocks)]
+        if not any(blocks):
+            return None
+        key = (tuple(sizes), tuple(blocks), rows, captured)
+        if self._plan[0] != key:
+            fill, (heads, kv_heads) = rows - len(seqs), self._heads()
+            self._plan = key, ops.shared_prefix(sizes + [1] * fill, blocks + [0] * fill, self.cache.block_size, heads, kv_heads, self.device,
+                                                ops.prefix_items(rows, kv_heads, self.device) if captured else 0)
+        return self._plan[1]
+
+    def _heads(self) -> Tuple[int, int]:
+        return self.cfg.num_attention_heads, self.cfg.kv_layout()[0][0]
+
     def grow(self, seqs: Sequence[_Seq]) -> None:
         """Extend the block list of sequences whose next token crosses a block boundary."""
         for s in seqs:
@@ -164,7 +272,7 @@ class NativeEngine:
         for s in seqs:
             self.cache.release(s.blocks)
             self.cache.release_slot(s.state_slot)
-            s.blocks, s.state_slot, s.linear = [], 0, {}
+            s.blocks, s.state_slot, s.linear, s.origin = [], 0, {}, None
 
     def _prompt_rows(self, seqs: Sequence[_Seq], lens: Sequence[int]) -> torch.Tensor:
         """Rows of the cache pools for packed prompts ``[ΣL]``, listed on the host and copied once."""
@@ -238,7 +346,7 @@ class NativeEngine:
 
     # --------------------------------------------------------------- decode
     def _decode_body(self, tokens, positions, table, seq_lens, lora: Optional[LoraBatch], seqs: Optional[List[_Seq]] = None,
-                     rope_positions: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None) -> torch.Tensor:
+                     rope_positions: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None, prefix: Optional[ops.SharedPrefix] = None) -> torch.Tensor:
         """One decode token per row from device tensors only (what a CUDA graph captures). Linear-attention layers of
         hybrid stacks keep their state on the sequences (``seqs``) and always run eagerly."""
         cfg, B = self.cfg, tokens.shape[0]
@@ -271,29 +379,36 @@ class NativeEngine:
                     continue
                 q, k, v, gate = at.heads_from(h, *(local if (local is not None and getattr(at, 'local_rope', False)) else (cos, sin)))
                 ops.cache_write(self.cache.k[li], self.cache.v[li], rows, *at.cache_entry(k, v))
-                o = ops.paged_attention_decode(q, self.cache.k[li], self.cache.v[li], table, seq_lens, at.scale,
-                                               window=getattr(at, 'window', None), softcap=getattr(at, 'softcap', None), sinks=getattr(at, 'sinks', None))
+                extras = {n: getattr(at, n, None) for n in ('window', 'softcap', 'sinks')}
+                if prefix is not None and q.shape[1] == prefix.heads and self.cache.k[li].shape[2] == prefix.kv_heads and not extras['window'] and not extras['softcap'] and extras['sinks'] is None:
+                    o = ops.paged_attention_shared(q, self.cache.k[li], self.cache.v[li], table, seq_lens, prefix, at.scale)
+                else:
+                    o = ops.paged_attention_decode(q, self.cache.k[li], self.cache.v[li], table, seq_lens, at.scale, **extras)
                 n, x = layer.after_attention(x, at.project_out(o, gate))
                 x = x + layer.feed_forward(n)
             x = self.model.norm(x)
         return self.model.logits(x).float()
 
-    def _graph_for(self, B: int, max_blocks: int):
-        """A captured decode step for batch bucket ``B`` and block-table width ``max_blocks`` (both powers of two).
+    def _graph_for(self, B: int, max_blocks: int, shared: bool = False):
+        """A captured decode step for batch bucket ``B`` and block-table width ``max_blocks`` (both powers of two); ``shared``: one that
+        reads shared prompts by a plan in static memory.
         Inputs live in static tensors that ``decode_step`` fills before every replay; rows beyond the live batch have
         length 0 and write their K/V into block 0, which no sequence owns."""
-        key = (B, max_blocks)
+        key = (B, max_blocks, shared)
         ent = self._graphs.get(key)
         if ent is not None:
             return ent
         dev = self.device
         ints = torch.zeros(B * (max_blocks + 2), dtype=torch.int32, device=dev)       # filled by one copy per step
         st = {'tokens': torch.zeros(B, dtype=torch.long, device=dev), 'ints': ints, 'table': ints[:B * max_blocks].view(B, max_blocks),
-              'seq_lens': ints[B * max_blocks:B * (max_blocks + 1)], 'slots': ints[B * (max_blocks + 1):]}
+              'seq_lens': ints[B * max_blocks:B * (max_blocks + 1)], 'slots': ints[B * (max_blocks + 1):], 'prefix': None, 'holds': None}
+        if shared:      # no piece of work yet; every plan of this batch fits
+            heads, kv_heads = self._heads()
+            st['prefix'] = ops.shared_prefix([1] * B, [0] * B, self.cache.block_size, heads, kv_heads, dev, ops.prefix_items(B, kv_heads, dev))
 
         def body():
             # the token of a step is the last of its sequence; rows that fill up the batch have length 0 and position 0
-            return self._decode_body(st['tokens'], (st['seq_lens'] - 1).clamp_min(0).long(), st['table'], st['seq_lens'], None, slots=st['slots'])
+            return self._decode_body(st['tokens'], (st['seq_lens'] - 1).clamp_min(0).long(), st['table'], st['seq_lens'], None, slots=st['slots'], prefix=st['prefix'])
 
         side = torch.cuda.Stream(device=dev)
         side.wait_stream(torch.cuda.current_stream(dev))
@@ -323,8 +438,9 @@ class NativeEngine:
         if use_graph:
             Bb = 1 << max(B - 1, 0).bit_length()
             Mb = 1 << max(max_blocks - 1, 0).bit_length()
+            prefix = self._shared(seqs, Bb, captured=True)
             try:
-                st = self._graph_for(Bb, Mb)
+                st = self._graph_for(Bb, Mb, prefix is not None)
             except Exception as e:  # capture is an optimisation: the eager path below is always valid
                 self.use_cuda_graphs = False
                 import logging
@@ -335,6 +451,9 @@ class NativeEngine:
                 ints = torch.empty(Bb * (Mb + 2), dtype=torch.int32, pin_memory=True)
                 ops.ext().pack_step(ints, Bb, Mb, [s.blocks for s in seqs], [s.length for s in seqs], [s.state_slot for s in seqs])
                 st['ints'].copy_(ints, non_blocking=True)
+                if prefix is not None and st['holds'] is not prefix:
+                    st['prefix'].plan.copy_(prefix.plan)
+                    st['holds'] = prefix
                 if B < Bb:
                     st['tokens'].zero_()
                 st['tokens'][:B].copy_(last_tokens)
@@ -349,7 +468,7 @@ class NativeEngine:
         deltas = [s.rope_delta for s in seqs]
         rope_pos = positions + torch.tensor(deltas, device=self.device) if any(deltas) else None
         slots = torch.tensor([s.state_slot for s in seqs], dtype=torch.int32, device=self.device)
-        logits = self._decode_body(last_tokens, positions, table, seq_lens, lora, seqs, rope_pos, slots)
+        logits = self._decode_body(last_tokens, positions, table, seq_lens, lora, seqs, rope_pos, slots, self._shared(seqs, B))
         if self.capture_routing:
             routed = self.model.collect_routed_experts()  # per layer [B, k]: the experts of the token just fed
             if routed is not None:
@@ -422,15 +541,36 @@ class NativeEngine:
             self._run_group(seqs[lo_i:lo_i + self.max_batch], responses, eos_token_id, on_token)
         return responses
 
+    def _start(self, seqs: List[_Seq]) -> Tuple[List[_Seq], torch.Tensor, List[int]]:
+        """Run the prompts; ``(sequences, hidden states, first row of every sequence in them)``.  With shared prompts each different one runs
+        once, and its sequences come one after the other."""
+        firsts, order = list(range(len(seqs))), list(range(len(seqs)))
+        if self.share_prompts:
+            seen: Dict[Any, int] = {}
+            for i, s in enumerate(seqs):
+                if s.vision is None:
+                    firsts[i] = seen.setdefault((tuple(s.prompt), s.slot, s.lora_rank, s.lora_scale, id(s.lora_target)), i)
+            order.sort(key=lambda i: (firsts[i], i))
+        run = [i for i in order if firsts[i] == i]
+        hidden = self.prefill([seqs[i] for i in run])
+        row, at = {}, 0
+        for i in run:
+            row[i] = at
+            at += len(seqs[i].prompt)
+        for i in run:
+            others = [seqs[j] for j in order if firsts[j] == i and j != i and not seqs[j].params.scoring_only]
+            if others:
+                self.fork(seqs[i], others)
+        return [seqs[i] for i in order], hidden, [row[firsts[i]] for i in order]
+
     def _run_group(self, seqs: List[_Seq], responses, eos, on_token) -> None:
-        hidden = self.prefill(seqs)
+        seqs, hidden, begins = self._start(seqs)
         lens = [len(s.prompt) for s in seqs]
-        ends = torch.tensor(lens, device=self.device).cumsum(0) - 1
+        ends = torch.tensor([a + n - 1 for a, n in zip(begins, lens)], device=self.device)
         # prompt scoring (teacher logprobs for distillation / max_tokens == 0)
         need_prompt = [s.params.prompt_logprobs is not None for s in seqs]
         if any(need_prompt):
-            off = 0
-            for s, n, need in zip(seqs, lens, need_prompt):
+            for s, off, n, need in zip(seqs, begins, lens, need_prompt):
                 if need and responses[s.request].prompt_logprobs is None:
                     h = hidden[off:off + n]
                     ids = torch.tensor(s.prompt[1:] + [0], device=self.device)
@@ -443,7 +583,6 @@ class NativeEngine:
                         v, ix = lg.topk(min(k, lg.shape[-1]), -1)
                         responses[s.request].topk_prompt_logprobs = [None] + [[(int(a), float(b)) for a, b in zip(r_i, r_v)]
                                                                              for r_i, r_v in zip(ix.tolist(), v.tolist())]
-                off += n
         live = [s for s in seqs if not s.params.scoring_only]
         for s in seqs:
             if s.params.scoring_only:

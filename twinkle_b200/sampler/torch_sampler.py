@@ -66,7 +66,8 @@ class TorchSampler(Sampler, CheckpointEngineMixin):
         ea = dict(engine_args or {})
         self.engine = NativeEngine(self.model, self.config, self.device, num_blocks=ea.get('num_blocks'),
                                    block_size=ea.get('block_size', 16), max_batch=ea.get('max_batch', 256),
-                                   gpu_memory_utilization=ea.get('gpu_memory_utilization', 0.85), decode=self._decode_tokens)
+                                   gpu_memory_utilization=ea.get('gpu_memory_utilization', 0.85), decode=self._decode_tokens,
+                                   share_prompts=bool(ea.get('share_prompts', False)))
         self.seed = seed + Platform.get_rank()
         self._synced_adapter = '__synced__'
         self._path_adapters: Dict[str, str] = {}
