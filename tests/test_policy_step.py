@@ -182,7 +182,9 @@ def _engine(stack, tmp_path, where=('cpu', 'float32'), share=False, block_size=1
         if not (tmp_path / stack).exists():
             (tmp_path / stack).mkdir()
             oracle.write_checkpoint(path, oracle.CONFIGS[name], oracle.random_weights(oracle.CONFIGS[name], 0))
-    return TorchSampler(model_id=path, device=where[0], enable_lora=False, dtype=where[1], engine_args=args).engine
+    engine = TorchSampler(model_id=path, device=where[0], enable_lora=False, dtype=where[1], engine_args=args).engine
+    engine.share_from = 0            # however little there is to share
+    return engine
 
 
 def run_group(engine, samples=3, max_tokens=9):

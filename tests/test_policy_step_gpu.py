@@ -50,7 +50,7 @@ def test_shared_decode(E, sizes, prompts, answers, bs, hq, hkv, D, fill):
     plan = ops.shared_prefix(sizes, shared, bs, hq, hkv)
     before = E.launch_count()
     out = ops.paged_attention_shared(*x, plan)
-    assert E.launch_count() - before == (2 if any(shared) else 1)
+    assert E.launch_count() - before == (3 if any(shared) else 1)
     close(out, *attention(*x))
     assert torch.equal(out, ops.paged_attention_shared(*x, plan))
     assert not out[len(out) - fill:].any()
@@ -452,6 +452,7 @@ def test_a_policy_step_end_to_end(E):
         setattr(ops, n, counted)
     try:
         eng = NativeEngine(model, cfg, num_blocks=200, block_size=16, share_prompts=True)
+        eng.share_from = 0
         prompts = [[(7 * i + 3) % 900 for i in range(300)], [(3 * i + 1) % 900 for i in range(64)]]
         res = eng.generate(prompts, [SamplingParams(max_tokens=20, temperature=1.0, num_samples=4) for _ in prompts])
     finally:
@@ -516,6 +517,7 @@ def test_a_group_that_shrinks_and_is_compacted(E):
     steps = {}
     for share in (False, True):
         eng = NativeEngine(model, cfg, num_blocks=160, block_size=16, max_batch=8, share_prompts=share)
+        eng.share_from = 0
         seqs = [_Seq(0, list(prompt), SamplingParams(max_tokens=8)) for _ in range(6)] + [_Seq(1, prompt[:40], SamplingParams(max_tokens=8))]
         if share:
             eng.prefill([seqs[0], seqs[6]])

@@ -825,6 +825,8 @@ class SharedPrefix(NamedTuple):
     heads: int
     kv_heads: int
     block_size: int
+    shared: int               # fewest pages that a group which shares any shares
+    pieces: int               # of a sequence's prefix, at most
 
 
 def _prefix_items(sizes, blocks, block_size: int, group: int, kv_heads: int, sms: int):
@@ -875,7 +877,8 @@ def shared_prefix(sizes, blocks, block_size: int, heads: int, kv_heads: int, dev
     work, lines = _prefix_items(sizes, blocks, block_size, heads // kv_heads, kv_heads, ext().num_sms() if torch.device(device).type == 'cuda' else 148)
     room = max(len(work), items)
     flat = [x for w in work for x in w] + [0] * (8 * (room - len(work))) + [x for l in lines for x in l]
-    return SharedPrefix(torch.tensor(flat, dtype=torch.int32).to(device), room, room, len(lines), heads, kv_heads, block_size)
+    return SharedPrefix(torch.tensor(flat, dtype=torch.int32).to(device), room, room, len(lines), heads, kv_heads, block_size, min((b for b in blocks if b), default=0),
+                        max((l[2] for l in lines), default=0))
 
 
 def prefix_items(sequences: int, kv_heads: int, device='cuda') -> int:
@@ -892,10 +895,12 @@ def paged_attention_shared(q, k_cache, v_cache, block_tables, seq_lens, prefix: 
         raise ValueError(f'paged_attention_shared: a plan for {prefix.sequences} sequences of {prefix.heads} / {prefix.kv_heads} heads and pages of {prefix.block_size}, got q '
                          f'{tuple(q.shape)} and pools {tuple(k_cache.shape)}')
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else scale
-    if (_cuda(q) and prefix.items and q.shape[0] and q.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16 and k_cache.shape == v_cache.shape and q.shape[-1] in (64, 128)
-            and prefix.block_size % 8 == 0 and k_cache.is_contiguous() and v_cache.is_contiguous() and all(t.data_ptr() % 16 == 0 for t in (q, k_cache, v_cache))):
-        return ext().paged_attn_shared(q.contiguous(), k_cache, v_cache, block_tables.to(torch.int32).contiguous(), seq_lens.to(torch.int32).contiguous(), prefix.plan, prefix.items,
-                                       prefix.slots, scale)
+    if (prefix.items and scale > 0 and prefix.block_size % 8 == 0 and _cuda(q) and q.shape[0] and q.shape[2] in (64, 128) and k_cache.shape == v_cache.shape
+            and q.dtype == k_cache.dtype == v_cache.dtype == torch.bfloat16 and k_cache.is_contiguous() and v_cache.is_contiguous()
+            and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0):
+        ints = (t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous() for t in (block_tables, seq_lens))
+        return ext().paged_attn_shared(q.contiguous(), k_cache, v_cache, *ints, prefix.plan, prefix.items, prefix.slots, prefix.pieces,
+                                       max(block_tables.shape[1] - prefix.shared, 0) * prefix.block_size, scale)
     return paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, scale)
 
 
@@ -1128,25 +1133,6 @@ def _side_by_side(t):
     return t if t.dim() == 1 or t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
-class _PolicyLoss(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, logps, entropies, labels, advantages, old, reference, args, entropy_coef, ignore_index):
-        loss, stats, deriv, weight = ext().policy_loss_fwd(logps, labels, advantages, old, reference, entropies, *args, ignore_index, ctx.needs_input_grad[0])
-        ctx.save_for_backward(deriv, weight, labels)
-        ctx.args = (entropy_coef, ignore_index)
-        ctx.mark_non_differentiable(stats)
-        return loss, stats
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gloss, _gstats):
-        deriv, weight, labels = ctx.saved_tensors
-        need_lp, need_ent = ctx.needs_input_grad[:2]
-        grad, grad_ent = ext().policy_loss_bwd(gloss.float().contiguous(), deriv if need_lp else None, weight, labels, *ctx.args, need_ent)
-        return (grad if need_lp else None, grad_ent if need_ent else None) + (None, ) * 7
-
-
 def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entropies=None, ratio: str = 'token', surrogate: str = 'clip', reduce: str = 'sequence', epsilon: float = 0.2,
                 epsilon_high: Optional[float] = None, beta: float = 0.0, entropy_coef: float = 0.0, tau=(1.0, 1.0), denominator: float = 1.0, ignore_index: int = -100):
     """``(loss, stats)`` of a policy step; differentiable by ``logps`` and ``entropies``.
@@ -1169,28 +1155,11 @@ def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entro
     labels = _loss_rows('policy_loss', logps, labels, {'old_logps': old_logps, 'ref_logps': ref_logps, 'entropies': entropies}, {'advantages': advantages})
     constants = [t for t in (advantages, old_logps, ref_logps) if t is not None]
     if _cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not (torch.is_grad_enabled() and any(t.requires_grad for t in constants)):
-        args = (_POLICY['ratio'].index(ratio), _POLICY['surrogate'].index(surrogate), _POLICY['reduce'].index(reduce), float(epsilon), float(epsilon_high), float(beta), float(entropy_coef),
-                float(tau[0]), float(tau[1]), float(denominator))
-        return _PolicyLoss.apply(_side_by_side(logps), _side_by_side(entropies), _side_by_side(labels), *(_side_by_side(t) for t in (advantages, old_logps, ref_logps)), args,
-                                 float(entropy_coef), int(ignore_index))
-    return ref.policy_loss(logps, labels, advantages, old_logps, ref_logps, entropies, ratio, surrogate, reduce, epsilon, epsilon_high, beta, entropy_coef, tau, denominator, ignore_index)
-
-
-class _PreferenceLoss(torch.autograd.Function):
-
-    @staticmethod
-    def forward(ctx, logps, labels, reference, args, ignore_index):
-        loss, stats, coef = ext().preference_loss_fwd(logps, labels, reference, *args, ignore_index)
-        ctx.save_for_backward(coef, labels)
-        ctx.ignore_index = ignore_index
-        ctx.mark_non_differentiable(stats)
+        loss, stats = ext().policy_loss(_side_by_side(logps), _side_by_side(entropies), _side_by_side(labels), _side_by_side(advantages), _side_by_side(old_logps), _side_by_side(ref_logps),
+                                        _POLICY['ratio'].index(ratio), _POLICY['surrogate'].index(surrogate), _POLICY['reduce'].index(reduce), epsilon, epsilon_high, beta, entropy_coef, *tau,
+                                        denominator, ignore_index)
         return loss, stats
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gloss, _gstats):
-        coef, labels = ctx.saved_tensors
-        return ext().preference_loss_bwd(gloss.float().contiguous(), coef, labels, ctx.ignore_index), None, None, None, None
+    return ref.policy_loss(logps, labels, advantages, old_logps, ref_logps, entropies, ratio, surrogate, reduce, epsilon, epsilon_high, beta, entropy_coef, tau, denominator, ignore_index)
 
 
 def preference_loss(logps, labels, ref_logps=None, form: str = 'sigmoid', beta: float = 0.1, gamma: float = 0.0, label_smoothing: float = 0.0, nll_weight: float = 0.0,
@@ -1212,8 +1181,8 @@ def preference_loss(logps, labels, ref_logps=None, form: str = 'sigmoid', beta: 
     gamma, label_smoothing = (gamma if form in ('sigmoid', 'simpo', 'hinge', 'ipo') else 0.0), (label_smoothing if form in ('sigmoid', 'simpo') else 0.0)
     if (_cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16)
             and not (torch.is_grad_enabled() and ref_logps is not None and ref_logps.requires_grad)):
-        args = (_PREFERENCE.index(form), float(beta), float(gamma), float(label_smoothing), float(nll_weight))
-        return _PreferenceLoss.apply(_side_by_side(logps), _side_by_side(labels), _side_by_side(ref_logps), args, int(ignore_index))
+        loss, stats = ext().preference_loss(_side_by_side(logps), _side_by_side(labels), _side_by_side(ref_logps), _PREFERENCE.index(form), beta, gamma, label_smoothing, nll_weight, ignore_index)
+        return loss, stats
     return ref.preference_loss(logps, labels, ref_logps, form, beta, gamma, label_smoothing, nll_weight, ignore_index)
 
 

@@ -71,13 +71,11 @@ torch::Tensor mlstm_step(const torch::Tensor&, int64_t, int64_t, int64_t, int64_
 void set_gemm_pair(int64_t);
 void set_gemm_staged(int64_t);
 #ifndef TK_SERVING_ONLY
-torch::Tensor paged_attn_shared(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t, int64_t, double);
+torch::Tensor paged_attn_shared(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t, int64_t, int64_t, int64_t, double);
 void cache_copy(const std::vector<torch::Tensor>&, const std::vector<int64_t>&, const std::vector<int64_t>&, const std::vector<int64_t>&);
-std::vector<torch::Tensor> policy_loss_fwd(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&, const c10::optional<torch::Tensor>&,
-                                           const c10::optional<torch::Tensor>&, int64_t, int64_t, int64_t, double, double, double, double, double, double, double, int64_t, bool);
-std::vector<torch::Tensor> policy_loss_bwd(const torch::Tensor&, const c10::optional<torch::Tensor>&, const torch::Tensor&, const torch::Tensor&, double, int64_t, bool);
-std::vector<torch::Tensor> preference_loss_fwd(const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&, int64_t, double, double, double, double, int64_t);
-torch::Tensor preference_loss_bwd(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t);
+std::vector<torch::Tensor> policy_loss(const torch::Tensor&, const c10::optional<torch::Tensor>&, const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&,
+                                       const c10::optional<torch::Tensor>&, int64_t, int64_t, int64_t, double, double, double, double, double, double, double, int64_t);
+std::vector<torch::Tensor> preference_loss(const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&, int64_t, double, double, double, double, int64_t);
 torch::Tensor grouped_gemm_wgrad(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t);
 std::vector<torch::Tensor> rmsnorm_fwd(const torch::Tensor&, const torch::Tensor&, double, double, const c10::optional<torch::Tensor>&);
 std::vector<torch::Tensor> rmsnorm_bwd(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, double,
@@ -202,10 +200,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
 #ifndef TK_SERVING_ONLY
   m.def("paged_attn_shared", &tk::paged_attn_shared);
   m.def("cache_copy", &tk::cache_copy);
-  m.def("policy_loss_fwd", &tk::policy_loss_fwd);
-  m.def("policy_loss_bwd", &tk::policy_loss_bwd);
-  m.def("preference_loss_fwd", &tk::preference_loss_fwd);
-  m.def("preference_loss_bwd", &tk::preference_loss_bwd);
+  m.def("policy_loss", &tk::policy_loss);
+  m.def("preference_loss", &tk::preference_loss);
   m.def("grouped_gemm_wgrad", &tk::grouped_gemm_wgrad);
   m.def("rmsnorm_fwd", &tk::rmsnorm_fwd, py::arg("x"), py::arg("w"), py::arg("eps"), py::arg("offset"), py::arg("residual") = py::none());
   m.def("rmsnorm_bwd", &tk::rmsnorm_bwd, py::arg("g"), py::arg("x"), py::arg("w"), py::arg("rstd"), py::arg("offset"),

@@ -105,4 +105,20 @@ CUtensorMap make_tmap_3d(const void* base, uint64_t d0, uint64_t d1, uint64_t d2
   return m;
 }
 
+CUtensorMap make_tmap_5d(const void* base, const uint64_t (&dims)[5], const uint64_t (&strides)[4], const uint32_t (&box)[5]) {
+  CUtensorMap m;
+  cuuint64_t d[5], st[4];
+  cuuint32_t b[5], estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < 5; ++i) {
+    d[i] = dims[i];
+    b[i] = box[i];
+  }
+  for (int i = 0; i < 4; ++i) st[i] = strides[i] * 2;
+  TORCH_CHECK(reinterpret_cast<uintptr_t>(base) % 16 == 0 && st[0] % 16 == 0 && st[1] % 16 == 0 && st[2] % 16 == 0 && st[3] % 16 == 0, "TMA: base and pitches must be 16-byte aligned");
+  CUresult r = encode_fn()(&m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(base), d, st, b, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  TORCH_CHECK(r == CUDA_SUCCESS, "cuTensorMapEncodeTiled(5d) failed with code ", static_cast<int>(r));
+  return m;
+}
+
 }  // namespace tk

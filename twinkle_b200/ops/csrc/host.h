@@ -37,4 +37,7 @@ CUtensorMap make_tmap_2d(const void* base, uint64_t inner, uint64_t outer, uint6
 CUtensorMap make_tmap_3d(const void* base, uint64_t d0, uint64_t d1, uint64_t d2, uint64_t s1, uint64_t s2, uint32_t b0,
                          uint32_t b1, uint32_t b2, int elem_bytes = 2, bool swizzle128 = true);
 
+// 5-D variant for 16-bit elements: strides (in elements) of the dimensions behind the contiguous one.
+CUtensorMap make_tmap_5d(const void* base, const uint64_t (&dims)[5], const uint64_t (&strides)[4], const uint32_t (&box)[5]);
+
 }  // namespace tk

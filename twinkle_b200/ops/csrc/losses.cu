@@ -22,7 +22,7 @@
 namespace tk {
 
 namespace ls {
-constexpr int THREADS = 256, UNROLL = 4;
+constexpr int THREADS = 256, UNROLL = 4, HOLD = 32, CTAS = 4;      // tokens of a batch, tokens whose terms a thread keeps, CTAs of an SM
 }
 
 // e^x to 2^-21: the rounding of x / ln 2 is carried along.
@@ -48,14 +48,22 @@ __device__ __forceinline__ float exp_rest(float x) {
   return r * x * x;
 }
 
-// Which tokens count: labels other than `ignore`, or a mask of bytes.
+// Which tokens count: labels other than `ignore`, or a mask of bytes (ignore: 0).
 struct Tokens {
   const void* p;
   long ld;
   int64_t ignore;
   bool bytes;
-  __device__ __forceinline__ bool at(long b, int t) const {
-    return bytes ? reinterpret_cast<const uint8_t*>(p)[b * ld + t] != 0 : reinterpret_cast<const int64_t*>(p)[b * ld + t] != ignore;
+  // What stands at U tokens, `step` apart; those from S on read the last one.  Loads only, without a branch between them: nothing waits for the first before the last is asked for.
+  template <int U>
+  __device__ __forceinline__ void load(int64_t (&x)[U], long b, int t0, int step, int S) const {
+    if (bytes) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = reinterpret_cast<const uint8_t*>(p)[b * ld + min(t0 + u * step, S - 1)];
+    } else {
+#pragma unroll
+      for (int u = 0; u < U; ++u) x[u] = reinterpret_cast<const int64_t*>(p)[b * ld + min(t0 + u * step, S - 1)];
+    }
   }
 };
 // A row per sequence with unit stride, or (one) a number per row; null: none.
@@ -63,10 +71,15 @@ struct Rows {
   const float* p;
   long ld;
   bool one;
-  __device__ __forceinline__ float at(long b, int t) const { return p[b * ld + (one ? 0 : t)]; }
+  template <int U>
+  __device__ __forceinline__ void load(float (&x)[U], long b, int t0, int step, int S) const {
+    if (p == nullptr) return;
+#pragma unroll
+    for (int u = 0; u < U; ++u) x[u] = p[b * ld + (one ? 0 : min(t0 + u * step, S - 1))];
+  }
 };
 
-// Sums of N numbers over the threads of a cluster; every thread gets them.  `sh`: [warps + 1][N] of shared memory, which a second call may use again.
+// Sums of N numbers over the threads of a cluster; every thread gets them.  `sh`: [warps + 2][N] of shared memory, which a second call may use again.
 template <int N>
 __device__ __forceinline__ void cluster_sums(double (&x)[N], double (*sh)[N], int ctas) {
   namespace cg = cooperative_groups;
@@ -89,17 +102,18 @@ __device__ __forceinline__ void cluster_sums(double (&x)[N], double (*sh)[N], in
   if (ctas > 1) {
     const cg::cluster_group cluster = cg::this_cluster();
     cluster.sync();
+    if (threadIdx.x < N) {          // a thread per number: from every thread these reads cost more than the tokens
+      double s = 0.0;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      x[i] = 0.0;
-      for (int r = 0; r < ctas; ++r) x[i] += cluster.map_shared_rank(&sh[WARPS][0], r)[i];
+      for (int r = 0; r < 8; ++r) s += r < ctas ? cluster.map_shared_rank(&sh[WARPS][0], r)[threadIdx.x] : 0.0;
+      sh[WARPS + 1][threadIdx.x] = s;
     }
     cluster.sync();                 // nobody leaves, and nothing is overwritten, while it is read
   } else {
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < N; ++i) x[i] = sh[WARPS][i];
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) x[i] = sh[ctas > 1 ? WARPS + 1 : WARPS][i];
 }
 
 // ---------------------------------------------------------------- policy loss
@@ -153,87 +167,44 @@ __device__ __forceinline__ void surrogate(const Policy& p, const Ratio& x, float
   }
 }
 
-// One row per cluster.  Sequence ratios take a second pass over the row, whose inputs then come from L2.
-template <int RATIO, int KIND>
-__global__ void __launch_bounds__(ls::THREADS) policy_rows_kernel(const Policy p) {
-  using namespace ls;
-  __shared__ double sh[THREADS / 32 + 1][6];
-  const int ctas = gridDim.x, first = blockIdx.x * THREADS + threadIdx.x, step = ctas * THREADS;
-  const long b = blockIdx.y;
-  double s[6] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};    // loss, tokens, KL, below, above; sequence ratios: Σ log ratio
-  auto log_ratio = [&](int t, bool& inside) {
-    const double d = p.old.p != nullptr ? static_cast<double>(p.logps.at(b, t)) - static_cast<double>(p.old.at(b, t)) : static_cast<double>(p.logps.at(b, t)) - p.logps.at(b, t);
+// Inputs of a thread's next tokens, all asked for before the first is used.
+template <int U>
+struct Batch {
+  float logp[U], old[U], ref[U], ent[U], adv[U];
+  bool on[U];
+  __device__ __forceinline__ void load(const Policy& p, long b, int t0, int step) {
+    int64_t label[U];
+    p.tokens.load(label, b, t0, step, p.S);
+    p.logps.load(logp, b, t0, step, p.S);
+    p.old.load(old, b, t0, step, p.S);
+    p.ref.load(ref, b, t0, step, p.S);
+    p.ent.load(ent, b, t0, step, p.S);
+    p.adv.load(adv, b, t0, step, p.S);
+    if (p.old.p == nullptr) {
+#pragma unroll
+      for (int u = 0; u < U; ++u) old[u] = logp[u];
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) on[u] = t0 + u * step < p.S && label[u] != p.tokens.ignore;
+  }
+  __device__ __forceinline__ double log_ratio(int u, bool& inside) const {
+    const double d = static_cast<double>(logp[u]) - static_cast<double>(old[u]);
     inside = d >= -20.0 && d <= 20.0;
     return d < -20.0 ? -20.0 : d > 20.0 ? 20.0 : d;
-  };
+  }
   // terms that do not come from the ratio: their loss, and the derivative by the log-prob
-  auto others = [&](int t, float& f, float& by_logp) {
+  __device__ __forceinline__ void others(const Policy& p, int u, float& f, float& by_logp) const {
     if (p.ref.p != nullptr) {
-      const float d = static_cast<float>(static_cast<double>(p.ref.at(b, t)) - static_cast<double>(p.logps.at(b, t)));
+      const float d = static_cast<float>(static_cast<double>(ref[u]) - static_cast<double>(logp[u]));
       const float e2 = exp_rest(d);
       f += p.beta * e2;
       by_logp -= p.beta * (e2 + d);
     }
-    if (p.ent.p != nullptr) f -= p.entropy * p.ent.at(b, t);
-  };
-  if constexpr (RATIO == RATIO_TOKEN) {
-    for (int t = first; t < p.S; t += step) {
-      float g = 0.f;
-      if (p.tokens.at(b, t)) {
-        bool inside;
-        const Ratio x = ratio_of(p, log_ratio(t, inside));
-        float f, by_ratio, by_logp;
-        surrogate<KIND>(p, x, p.adv.at(b, t), p.logps.at(b, t), f, by_ratio, by_logp);
-        others(t, f, by_logp);
-        g = (inside ? by_ratio : 0.f) + by_logp;
-        s[0] += f;
-        s[1] += 1.0;
-        s[2] += exp_rest(x.lr);
-        s[3] += x.below;
-        s[4] += x.above;
-      }
-      if (p.deriv != nullptr) p.deriv[b * p.S + t] = g;
-    }
-    cluster_sums(s, sh, ctas);
-  } else {
-    for (int t = first; t < p.S; t += step)
-      if (p.tokens.at(b, t)) {
-        bool inside;
-        s[5] += log_ratio(t, inside);
-        s[1] += 1.0;
-      }
-    cluster_sums(s, sh, ctas);
-    const double n = s[1] > 0.0 ? s[1] : 1.0;
-    const Ratio x = ratio_of(p, s[5] / n);
-    double u[2] = {0.0, 0.0};        // loss, derivative by the row's log ratio
-    for (int t = first; t < p.S; t += step)
-      if (p.tokens.at(b, t)) {
-        float f, by_ratio, by_logp;
-        surrogate<KIND>(p, x, p.adv.at(b, t), p.logps.at(b, t), f, by_ratio, by_logp);
-        others(t, f, by_logp);
-        u[0] += f;
-        u[1] += by_ratio;
-      }
-    cluster_sums(u, reinterpret_cast<double(*)[2]>(&sh[0][0]), ctas);
-    const float by_each = static_cast<float>(u[1] / n);
-    if (p.deriv != nullptr)
-      for (int t = first; t < p.S; t += step) {
-        float g = 0.f;
-        if (p.tokens.at(b, t)) {
-          bool inside;
-          log_ratio(t, inside);
-          float f, by_ratio, by_logp;
-          surrogate<KIND>(p, x, p.adv.at(b, t), p.logps.at(b, t), f, by_ratio, by_logp);
-          others(t, f, by_logp);
-          g = (inside ? by_each : 0.f) + by_logp;
-        }
-        p.deriv[b * p.S + t] = g;
-      }
-    s[0] = u[0];
-    s[2] = s[1] * static_cast<double>(exp_rest(x.lr));
-    s[3] = x.below ? s[1] : 0.0;
-    s[4] = x.above ? s[1] : 0.0;
+    if (p.ent.p != nullptr) f -= p.entropy * ent[u];
   }
+};
+
+__device__ __forceinline__ void put_sums(const Policy& p, long b, const double (&s)[5]) {
   if (blockIdx.x == 0 && threadIdx.x < 5) {
     double v = s[0];
 #pragma unroll
@@ -242,11 +213,125 @@ __global__ void __launch_bounds__(ls::THREADS) policy_rows_kernel(const Policy p
   }
 }
 
+// Ratios of tokens; one row per cluster.
+template <int KIND>
+__global__ void __launch_bounds__(ls::THREADS, ls::CTAS) policy_token_kernel(const Policy p) {
+  using namespace ls;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ double sh[THREADS / 32 + 2][5];
+  const int ctas = gridDim.x, step = ctas * THREADS;
+  const long b = blockIdx.y;
+  double loss = 0.0, kl = 0.0;
+  int n = 0, below = 0, above = 0;
+  for (int t0 = blockIdx.x * THREADS + threadIdx.x; t0 < p.S; t0 += step * UNROLL) {
+    Batch<UNROLL> x;
+    x.load(p, b, t0, step);
+    float f4 = 0.f, kl4 = 0.f;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      float g = 0.f;
+      if (x.on[u]) {
+        bool inside;
+        const Ratio r = ratio_of(p, x.log_ratio(u, inside));
+        float f, by_ratio, by_logp;
+        surrogate<KIND>(p, r, x.adv[u], x.logp[u], f, by_ratio, by_logp);
+        x.others(p, u, f, by_logp);
+        g = (inside ? by_ratio : 0.f) + by_logp;
+        f4 += f;
+        kl4 += exp_rest(r.lr);
+        ++n;
+        below += r.below;
+        above += r.above;
+      }
+      if (p.deriv != nullptr && t0 + u * step < p.S) p.deriv[b * p.S + t0 + u * step] = g;
+    }
+    loss += f4;
+    kl += kl4;
+  }
+  double s[5] = {loss, static_cast<double>(n), kl, static_cast<double>(below), static_cast<double>(above)};
+  cluster_sums(s, sh, ctas);
+  put_sums(p, b, s);
+}
+
+// One ratio per row.  The row's loss and its derivative by the logarithm of the ratio are sums over the advantages of either sign, so one pass over the inputs is enough; what a token's
+// own derivative needs beside them stays in shared memory for rows of up to HOLD tokens per thread of the cluster, and comes from the inputs again, then in L2, for longer ones.
+template <int KIND>
+__global__ void __launch_bounds__(ls::THREADS, ls::CTAS) policy_sequence_kernel(const Policy p) {
+  using namespace ls;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  __shared__ double sh[THREADS / 32 + 2][6];
+  const int ctas = gridDim.x, step = ctas * THREADS, first = blockIdx.x * THREADS + threadIdx.x;
+  const long b = blockIdx.y;
+  const bool held = KIND != WEIGHT && p.S <= step * HOLD;
+  __shared__ float keep[HOLD][THREADS];
+  uint32_t on = 0, inner = 0;
+  double s[6] = {0.0, 0.0, 0.0, 0.0, 0.0, 0.0};      // other terms, tokens, log ratios, advantages from 0 on, below 0, advantage · log-prob
+  auto sum = [&](int t0, int at) {
+    Batch<UNROLL> x;
+    x.load(p, b, t0, step);
+    float f4 = 0.f;
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (x.on[u]) {
+        bool inside;
+        s[2] += x.log_ratio(u, inside);
+        float by_logp = 0.f;
+        x.others(p, u, f4, by_logp);
+        s[1] += 1.0;
+        if (x.adv[u] >= 0.f) s[3] += x.adv[u]; else s[4] += x.adv[u];
+        if constexpr (KIND == WEIGHT) s[5] += static_cast<double>(x.adv[u]) * x.logp[u];
+        if (held) {
+          keep[at + u][threadIdx.x] = by_logp;
+          on |= 1u << (at + u);
+          inner |= (inside ? 1u : 0u) << (at + u);
+        }
+      }
+    s[0] += f4;
+  };
+  for (int t0 = first, at = 0; t0 < p.S; t0 += step * UNROLL, at += UNROLL) sum(t0, at);
+  cluster_sums(s, sh, ctas);
+  const double n = s[1] > 0.0 ? s[1] : 1.0;
+  const Ratio r = ratio_of(p, s[2] / n);
+  // the surrogate is proportional to the size of the advantage
+  float f_up, d_up, f_down, d_down, by_logp;
+  surrogate<KIND>(p, r, 1.f, 0.f, f_up, d_up, by_logp);
+  surrogate<KIND>(p, r, -1.f, 0.f, f_down, d_down, by_logp);
+  const float weight = r.over ? p.top : r.r;
+  const double loss = s[0] + (KIND == WEIGHT ? -weight * s[5] : f_up * s[3] - f_down * s[4]);
+  const float by_each = KIND == WEIGHT ? 0.f : static_cast<float>((d_up * s[3] - d_down * s[4]) / n);
+  if (p.deriv != nullptr) {
+    if (held) {
+#pragma unroll 4
+      for (int t = first, i = 0; t < p.S; t += step, ++i) p.deriv[b * p.S + t] = on >> i & 1u ? (inner >> i & 1u ? by_each : 0.f) + keep[i][threadIdx.x] : 0.f;
+    } else {
+      for (int t0 = first; t0 < p.S; t0 += step * UNROLL) {
+        Batch<UNROLL> x;
+        x.load(p, b, t0, step);
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+          float g = 0.f;
+          if (x.on[u]) {
+            bool inside;
+            x.log_ratio(u, inside);
+            float f = 0.f, direct = KIND == WEIGHT ? -weight * x.adv[u] : 0.f;
+            x.others(p, u, f, direct);
+            g = (inside ? by_each : 0.f) + direct;
+          }
+          if (t0 + u * step < p.S) p.deriv[b * p.S + t0 + u * step] = g;
+        }
+      }
+    }
+  }
+  const double out[5] = {loss, s[1], s[1] * static_cast<double>(exp_rest(r.lr)), r.below ? s[1] : 0.0, r.above ? s[1] : 0.0};
+  put_sums(p, b, out);
+}
+
 // Joins the rows: loss, weight of every row, figures.  One CTA; threads take rows in turn, so the order of the sums is that of the rows' numbers.
 __global__ void __launch_bounds__(ls::THREADS) policy_join_kernel(const double* __restrict__ sums, float* __restrict__ weight, float* __restrict__ loss, float* __restrict__ stats, int B,
                                                                   int reduce, double denominator) {
-  __shared__ double sh[ls::THREADS / 32 + 1][5];
+  __shared__ double sh[ls::THREADS / 32 + 2][5];
   double s[5] = {0.0, 0.0, 0.0, 0.0, 0.0};
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int b = threadIdx.x; b < B; b += ls::THREADS) {
     const double n = sums[b * 5L + 1] > 0.0 ? sums[b * 5L + 1] : 1.0;
     s[0] += reduce == REDUCE_SEQUENCE ? sums[b * 5L] / n : sums[b * 5L];
@@ -271,11 +356,22 @@ __global__ void __launch_bounds__(ls::THREADS) policy_join_kernel(const double* 
 // grad = derivative · weight of the row · gradient of the loss; entropies: −c · weight · gradient of the loss on tokens that count
 __global__ void __launch_bounds__(ls::THREADS) policy_grad_kernel(const float* __restrict__ deriv, const float* __restrict__ weight, const float* __restrict__ up, const Tokens tokens,
                                                                   float entropy, float* __restrict__ grad, float* __restrict__ grad_ent, int S) {
+  using namespace ls;
   const long b = blockIdx.y;
   const float w = weight[b] * *up;
-  for (int t = blockIdx.x * ls::THREADS + threadIdx.x; t < S; t += gridDim.x * ls::THREADS) {
-    if (grad != nullptr) grad[b * S + t] = deriv[b * S + t] * w;
-    if (grad_ent != nullptr) grad_ent[b * S + t] = tokens.at(b, t) ? -entropy * w : 0.f;
+  const int step = gridDim.x * THREADS;
+  for (int t0 = blockIdx.x * THREADS + threadIdx.x; t0 < S; t0 += step * UNROLL) {
+    float d[UNROLL];
+    int64_t label[UNROLL];
+    if (grad != nullptr) Rows{deriv, S, false}.load(d, b, t0, step, S);
+    if (grad_ent != nullptr) tokens.load(label, b, t0, step, S);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u) {
+      const int t = t0 + u * step;
+      if (t >= S) break;
+      if (grad != nullptr) grad[b * S + t] = d[u] * w;
+      if (grad_ent != nullptr) grad_ent[b * S + t] = label[u] != tokens.ignore ? -entropy * w : 0.f;
+    }
   }
 }
 
@@ -289,23 +385,36 @@ struct Preference {
   int S;
 };
 
-__global__ void __launch_bounds__(ls::THREADS) preference_rows_kernel(const Preference p) {
+__global__ void __launch_bounds__(ls::THREADS, ls::CTAS) preference_rows_kernel(const Preference p) {
   using namespace ls;
-  __shared__ double sh[THREADS / 32 + 1][3];
+  __shared__ double sh[THREADS / 32 + 2][3];
   const int ctas = gridDim.x;
   const long b = blockIdx.y;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int step = ctas * THREADS;
+  const bool each = p.ref.p != nullptr && !p.ref.one;
   double s[3] = {0.0, 0.0, 0.0};
-  for (int t = blockIdx.x * THREADS + threadIdx.x; t < p.S; t += ctas * THREADS)
-    if (p.tokens.at(b, t)) {
-      s[0] += p.logps.at(b, t);
-      s[1] += 1.0;
-      if (p.ref.p != nullptr && !p.ref.one) s[2] += p.ref.at(b, t);
-    }
+  int n = 0;
+  for (int t0 = blockIdx.x * THREADS + threadIdx.x; t0 < p.S; t0 += step * UNROLL) {
+    float x[UNROLL], y[UNROLL] = {};
+    int64_t label[UNROLL];
+    p.tokens.load(label, b, t0, step, p.S);
+    p.logps.load(x, b, t0, step, p.S);
+    if (each) p.ref.load(y, b, t0, step, p.S);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (t0 + u * step < p.S && label[u] != p.tokens.ignore) {
+        s[0] += x[u];
+        s[2] += y[u];
+        ++n;
+      }
+  }
+  s[1] = n;
   cluster_sums(s, sh, ctas);
   if (blockIdx.x == 0 && threadIdx.x == 0) {
     p.sums[b * 3] = s[0];
     p.sums[b * 3 + 1] = s[1];
-    p.sums[b * 3 + 2] = p.ref.p != nullptr && p.ref.one ? static_cast<double>(p.ref.at(b, 0)) : s[2];
+    p.sums[b * 3 + 2] = p.ref.p != nullptr && p.ref.one ? static_cast<double>(p.ref.p[b * p.ref.ld]) : s[2];
   }
 }
 
@@ -317,12 +426,13 @@ struct PairArgs {
 __device__ __forceinline__ double softplus64(double z) { return fmax(z, 0.0) + log1p(exp(-fabs(z))); }
 __device__ __forceinline__ double sigmoid64(double z) { return 1.0 / (1.0 + exp(-z)); }
 
-__global__ void __launch_bounds__(ls::THREADS) preference_join_kernel(const double* __restrict__ sums, const PairArgs a, float* __restrict__ coef, float* __restrict__ loss,
+__global__ void __launch_bounds__(ls::THREADS) preference_join_kernel(const double* __restrict__ sums, PairArgs a, float* __restrict__ coef, float* __restrict__ loss,
                                                                       float* __restrict__ stats) {
-  __shared__ double sh[ls::THREADS / 32 + 1][7];
+  __shared__ double sh[ls::THREADS / 32 + 2][7];
   double s[7] = {};     // losses, chosen and rejected levels, chosen above rejected, log-probs of both, chosen tokens
   const bool mean = a.form == SIMPO || a.form == ORPO;
   double chosen_tokens = 0.0;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   // the likelihood term's denominator is a sum over all pairs: it comes first
   if (a.nll != 0.0) {
     double n[1] = {0.0};
@@ -385,16 +495,25 @@ __global__ void __launch_bounds__(ls::THREADS) preference_join_kernel(const doub
 }
 
 __global__ void __launch_bounds__(ls::THREADS) preference_grad_kernel(const float* __restrict__ coef, const float* __restrict__ up, const Tokens tokens, float* __restrict__ grad, int S) {
+  using namespace ls;
   const long b = blockIdx.y;
   const float c = coef[b] * *up;
-  for (int t = blockIdx.x * ls::THREADS + threadIdx.x; t < S; t += gridDim.x * ls::THREADS) grad[b * S + t] = tokens.at(b, t) ? c : 0.f;
+  const int step = gridDim.x * THREADS;
+  for (int t0 = blockIdx.x * THREADS + threadIdx.x; t0 < S; t0 += step * UNROLL) {
+    int64_t label[UNROLL];
+    tokens.load(label, b, t0, step, S);
+#pragma unroll
+    for (int u = 0; u < UNROLL; ++u)
+      if (t0 + u * step < S) grad[b * S + t0 + u * step] = label[u] != tokens.ignore ? c : 0.f;
+  }
 }
 
 // -------------------------------------------------------------------- host side
-static Tokens tokens_of(const torch::Tensor& labels, const torch::Tensor& logps, int64_t ignore) {
-  TORCH_CHECK(labels.is_cuda() && labels.device() == logps.device() && labels.sizes() == logps.sizes() && (labels.scalar_type() == torch::kInt64 || labels.scalar_type() == torch::kBool) &&
+static Tokens tokens_of(const torch::Tensor& labels, const torch::Tensor& like, int64_t ignore) {
+  TORCH_CHECK(labels.is_cuda() && labels.device() == like.device() && labels.sizes() == like.sizes() && (labels.scalar_type() == torch::kInt64 || labels.scalar_type() == torch::kBool) &&
                   (labels.size(1) <= 1 || labels.stride(1) == 1), "labels int64 or a boolean mask [rows, tokens] like the log-probs, tokens side by side");
-  return {labels.data_ptr(), labels.stride(0), ignore, labels.scalar_type() == torch::kBool};
+  const bool bytes = labels.scalar_type() == torch::kBool;
+  return {labels.data_ptr(), labels.stride(0), bytes ? 0 : ignore, bytes};
 }
 static Rows rows_of(const OptT& t, const torch::Tensor& like, bool per_row, const char* what) {
   if (!has(t)) return {nullptr, 0, false};
@@ -412,10 +531,11 @@ static void check_logps(const torch::Tensor& logps) {
   TORCH_CHECK(logps.size(0) <= 65535 && logps.size(1) < (int64_t(1) << 30), "up to 65535 rows of 2^30 tokens");
 }
 
-// CTAs per row: as many as give every SM two, with a pass of the CTA's threads or more for each.
+// CTAs per row: down to a batch of tokens per thread, while all are resident at once (more of them, each with less to do, wait for one another's latencies: 256 rows of 16k tokens
+// took 80 us on 8 CTAs a row).
 static int row_ctas(int64_t B, int64_t S) {
   int c = 1;
-  while (c < 8 && B * c < 2 * num_sms() && S > static_cast<int64_t>(c) * ls::THREADS * ls::UNROLL) c *= 2;
+  while (c < 8 && 2 * B * c <= ls::CTAS * num_sms() && S > static_cast<int64_t>(c) * ls::THREADS * ls::UNROLL) c *= 2;
   return c;
 }
 
@@ -434,8 +554,23 @@ static void launch_rows(F kernel, const P& p, int64_t B, int64_t S, cudaStream_t
   TK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
   count_launch();
 }
+// Joins the rows: begins while they are summed and waits for them.
+template <typename... A>
+static void launch_join(void (*kernel)(A...), cudaStream_t stream, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(1);
+  cfg.blockDim = dim3(ls::THREADS);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  count_launch();
+}
 static dim3 grad_grid(int64_t B, int64_t S) {
-  const int64_t most = (8 * num_sms() + B - 1) / B, want = (S + ls::THREADS - 1) / ls::THREADS;
+  const int64_t most = (8 * num_sms() + B - 1) / B, want = (S + ls::THREADS * ls::UNROLL - 1) / (ls::THREADS * ls::UNROLL);
   return dim3(static_cast<unsigned>(std::max<int64_t>(1, std::min(want, most))), static_cast<unsigned>(B));
 }
 
@@ -466,13 +601,12 @@ std::vector<torch::Tensor> policy_loss_fwd(const torch::Tensor& logps, const tor
   auto stream = at::cuda::getCurrentCUDAStream();
   auto go = [&](auto kernel) { launch_rows(kernel, p, B, S, stream); };
   if (ratio == RATIO_TOKEN) {
-    if (kind == CLIP) go(policy_rows_kernel<RATIO_TOKEN, CLIP>); else if (kind == SOFT) go(policy_rows_kernel<RATIO_TOKEN, SOFT>); else go(policy_rows_kernel<RATIO_TOKEN, WEIGHT>);
+    if (kind == CLIP) go(policy_token_kernel<CLIP>); else if (kind == SOFT) go(policy_token_kernel<SOFT>); else go(policy_token_kernel<WEIGHT>);
   } else {
-    if (kind == CLIP) go(policy_rows_kernel<RATIO_SEQUENCE, CLIP>); else if (kind == SOFT) go(policy_rows_kernel<RATIO_SEQUENCE, SOFT>); else go(policy_rows_kernel<RATIO_SEQUENCE, WEIGHT>);
+    if (kind == CLIP) go(policy_sequence_kernel<CLIP>); else if (kind == SOFT) go(policy_sequence_kernel<SOFT>); else go(policy_sequence_kernel<WEIGHT>);
   }
-  policy_join_kernel<<<1, ls::THREADS, 0, stream>>>(p.sums, weight.data_ptr<float>(), loss.data_ptr<float>(), stats.data_ptr<float>(), static_cast<int>(B), static_cast<int>(reduce), denominator);
-  count_launch();
-  TK_CUDA_CHECK(cudaGetLastError());
+  launch_join(policy_join_kernel, stream, static_cast<const double*>(p.sums), weight.data_ptr<float>(), loss.data_ptr<float>(), stats.data_ptr<float>(), static_cast<int>(B), static_cast<int>(reduce),
+              denominator);
   return {loss, stats, deriv, weight};
 }
 
@@ -483,7 +617,7 @@ std::vector<torch::Tensor> policy_loss_bwd(const torch::Tensor& up, const OptT& 
   const int64_t B = labels.size(0), S = labels.size(1);
   const auto f32 = weight.options();
   auto grad = has(deriv) ? torch::empty({B, S}, f32) : torch::empty({0}, f32), grad_ent = want_ent ? torch::empty({B, S}, f32) : torch::empty({0}, f32);
-  const Tokens tokens{labels.data_ptr(), labels.stride(0), ignore, labels.scalar_type() == torch::kBool};
+  const Tokens tokens = tokens_of(labels, labels, ignore);
   policy_grad_kernel<<<grad_grid(B, S), ls::THREADS, 0, at::cuda::getCurrentCUDAStream()>>>(has(deriv) ? deriv->data_ptr<float>() : nullptr, weight.data_ptr<float>(), up.data_ptr<float>(), tokens,
       static_cast<float>(entropy), has(deriv) ? grad.data_ptr<float>() : nullptr, want_ent ? grad_ent.data_ptr<float>() : nullptr, static_cast<int>(S));
   count_launch();
@@ -509,9 +643,7 @@ std::vector<torch::Tensor> preference_loss_fwd(const torch::Tensor& logps, const
   auto stream = at::cuda::getCurrentCUDAStream();
   launch_rows(preference_rows_kernel, p, B, S, stream);
   const PairArgs a{static_cast<int>(form), static_cast<int>(B / 2), beta, gamma, smoothing, nll};
-  preference_join_kernel<<<1, ls::THREADS, 0, stream>>>(p.sums, a, coef.data_ptr<float>(), loss.data_ptr<float>(), stats.data_ptr<float>());
-  count_launch();
-  TK_CUDA_CHECK(cudaGetLastError());
+  launch_join(preference_join_kernel, stream, static_cast<const double*>(p.sums), a, coef.data_ptr<float>(), loss.data_ptr<float>(), stats.data_ptr<float>());
   return {loss, stats, coef};
 }
 
@@ -520,7 +652,7 @@ torch::Tensor preference_loss_bwd(const torch::Tensor& up, const torch::Tensor& 
   c10::cuda::CUDAGuard guard(coef.device());
   const int64_t B = labels.size(0), S = labels.size(1);
   auto grad = torch::empty({B, S}, coef.options());
-  const Tokens tokens{labels.data_ptr(), labels.stride(0), ignore, labels.scalar_type() == torch::kBool};
+  const Tokens tokens = tokens_of(labels, labels, ignore);
   preference_grad_kernel<<<grad_grid(B, S), ls::THREADS, 0, at::cuda::getCurrentCUDAStream()>>>(coef.data_ptr<float>(), up.data_ptr<float>(), tokens, grad.data_ptr<float>(), static_cast<int>(S));
   count_launch();
   TK_CUDA_CHECK(cudaGetLastError());

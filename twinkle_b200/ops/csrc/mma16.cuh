@@ -21,6 +21,12 @@ __device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint3
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {   // zeros when not live
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
+}
+
+// A sum from leading parts and remainders.  An infinite value meets a positive leading part, and a remainder that is zero or negative: the leading sum is the result.
+__device__ __forceinline__ float whole(float lead, float rest) { return fabsf(lead) == INFINITY ? lead : lead + rest; }
 // two values as bf16 pairs: the rounded ones and what the rounding left over
 __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& lo) {
   hi = pack_bf16(x, y);

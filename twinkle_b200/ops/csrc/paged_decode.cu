@@ -36,17 +36,8 @@ template <int D> constexpr int stage_bytes() { return 2 * TILE * row_bytes<D>();
 template <int D> constexpr int smem_bytes() { return WARPS * STAGES * stage_bytes<D>(); }
 }  // namespace pd
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool live) {   // zeros when not live
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
-}
-
-// A sum from leading parts and remainders.  An infinite value meets a positive leading part, and a remainder that is zero or negative: the leading sum is the result.
-__device__ __forceinline__ float whole(float lead, float rest) { return fabsf(lead) == INFINITY ? lead : lead + rest; }
-
-// JOIN: the keys of a shared prefix are left out, what paged_shared.cu found there comes in at the end.  A sequence shorter than its group's prefix has no part in it and
-// reads all of its own keys.
-template <int D, bool JOIN>
-__global__ void __launch_bounds__(pd::WARPS * 32, 2) paged_decode_mma_kernel(const PagedDecode p, const PagedJoin join) {
+template <int D>
+__global__ void __launch_bounds__(pd::WARPS * 32, 2) paged_decode_mma_kernel(const PagedDecode p) {
   using namespace pd;
   namespace cg = cooperative_groups;
   constexpr int CH = D / 8;                 // 16-byte chunks of a row
@@ -55,17 +46,7 @@ __global__ void __launch_bounds__(pd::WARPS * 32, 2) paged_decode_mma_kernel(con
   const int S = gridDim.x, split = blockIdx.x, b = blockIdx.z;
   const int groups = (p.G + HEADS - 1) / HEADS, kvh = blockIdx.y / groups, g0 = blockIdx.y % groups * HEADS, h0 = kvh * p.G + g0, GH = min(HEADS, p.G - g0);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, hrow = lane >> 2;
-  const int n = p.seq_lens[b];
-  int first = n > 0 ? first_visible(n - 1, p.window, p.chunk) : 0, slot0 = 0, slots = 0, slot_row = 0;
-  if constexpr (JOIN) {
-    const int4 r = reinterpret_cast<const int4*>(join.rows)[b];
-    if (n >= r.x && r.x >= 0 && r.z > 0 && r.y >= 0 && r.y + r.z <= join.slots && r.w >= 0 && r.w + p.G <= 128) {
-      first = r.x;
-      slot0 = r.y;
-      slots = r.z;
-      slot_row = r.w;
-    }
-  }
+  const int n = p.seq_lens[b], first = n > 0 ? first_visible(n - 1, p.window, p.chunk) : 0;
   const int base = first & ~(TILE - 1), tiles = n > base ? (n - base + TILE - 1) / TILE : 0, workers = S * WARPS, worker = split * WARPS + warp;
   const int mine = tiles > worker ? (tiles - worker + workers - 1) / workers : 0;
 
@@ -78,14 +59,7 @@ __global__ void __launch_bounds__(pd::WARPS * 32, 2) paged_decode_mma_kernel(con
   auto lookup = [&](int i) -> int {
     const int t = base + (worker + i * workers) * TILE + (lane & 15);
     if (i >= mine || t >= n || t < first) return -1;
-    const int block = table[t / p.block_size];
-    if constexpr (JOIN) {
-      if (block < 0 || block >= join.num_blocks) {      // whoever reads the word next raises
-        atomicCAS(join.err, 0, ERR_BOUNDS);
-        return -1;
-      }
-    }
-    return block * p.block_size + t % p.block_size;
+    return table[t / p.block_size] * p.block_size + t % p.block_size;
   };
   auto fetch = [&](int i, int rows) {
     const uint32_t dst = smem_u32(ring) + (i % STAGES) * stage_bytes<D>();
@@ -218,24 +192,13 @@ __global__ void __launch_bounds__(pd::WARPS * 32, 2) paged_decode_mma_kernel(con
     }
   }
   if (S > 1) cluster.sync(); else __syncthreads();
-  if constexpr (JOIN) asm volatile("griddepcontrol.wait;" ::: "memory");      // the prefixes are done
   // CTA r of the cluster finishes every S-th stretch of 128 results
   for (int i = split * WARPS * 32 + threadIdx.x; i < GH * D; i += S * WARPS * 32) {
     const int h = i / D;
     float mm = -INFINITY, sink = 0.f;
     if (p.sinks != nullptr) mm = sink = __bfloat162float(reinterpret_cast<const bf16*>(p.sinks)[h0 + h]) * 1.4426950408889634f;
     for (int r = 0; r < S; ++r) mm = fmaxf(mm, cluster.map_shared_rank(top, r)[h]);
-    const size_t found = JOIN ? (static_cast<size_t>(slot0) * p.hkv + kvh) * 128 + slot_row + g0 + h : 0, next = static_cast<size_t>(p.hkv) * 128;
-    if constexpr (JOIN)
-      for (int k = 0; k < slots; ++k) mm = fmaxf(mm, join.stat[found + k * next].x);
     float o = 0.f, ll = p.sinks != nullptr ? fast_exp2(sink - mm) : 0.f;
-    if constexpr (JOIN)
-      for (int k = 0; k < slots; ++k) {
-        const float2 t = join.stat[found + k * next];
-        const float c = t.x == -INFINITY ? 0.f : fast_exp2(t.x - mm);
-        o += join.part[(found + k * next) * D + i % D] * c;
-        ll += t.y * c;
-      }
     for (int r = 0; r < S; ++r) {
       const float* t = cluster.map_shared_rank(top, r);
       const float mr = t[h], c = mr == -INFINITY ? 0.f : fast_exp2(mr - mm);
@@ -259,25 +222,23 @@ static int cluster_size(const PagedDecode& p, int B, int groups) {
   return S;
 }
 
-template <int D, bool JOIN>
-static void launch(const PagedDecode& p, const PagedJoin& join, int B, cudaStream_t stream) {
+template <int D>
+static void launch(const PagedDecode& p, int B, cudaStream_t stream) {
   static OncePerDevice limit;
-  limit(current_device(), [] { TK_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_mma_kernel<D, JOIN>, cudaFuncAttributeMaxDynamicSharedMemorySize, pd::smem_bytes<D>())); });
+  limit(current_device(), [] { TK_CUDA_CHECK(cudaFuncSetAttribute(paged_decode_mma_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, pd::smem_bytes<D>())); });
   const int groups = (p.G + pd::HEADS - 1) / pd::HEADS, S = cluster_size(p, B, groups);
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(S, p.hkv * groups, B);
   cfg.blockDim = dim3(pd::WARPS * 32);
   cfg.dynamicSmemBytes = pd::smem_bytes<D>();
   cfg.stream = stream;
-  cudaLaunchAttribute attr[2]{};
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = S;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = JOIN ? 2 : 1;
-  TK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_decode_mma_kernel<D, JOIN>, p, join));
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = S;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_decode_mma_kernel<D>, p));
 }
 
 bool paged_decode_mma(const PagedDecode& p, int B, int d, int e, cudaStream_t stream) {
@@ -287,13 +248,8 @@ bool paged_decode_mma(const PagedDecode& p, int B, int d, int e, cudaStream_t st
   // decoders that have such groups are small and deep, and any other order of these sums moves the logits of a 28-layer stack by 2.7–3.8 %, at the same
   // distance from 64 bits (3.7–4.1 %).  perf/cases.py grants such stacks 3 %, so their steps keep the order that they had.
   if (!aligned || p.G < 4 || d != e || (d != 64 && d != 128) || B > 65535 || p.hkv * ((p.G + pd::HEADS - 1) / pd::HEADS) > 65535) return false;
-  if (d == 64) launch<64, false>(p, PagedJoin{}, B, stream); else launch<128, false>(p, PagedJoin{}, B, stream);
+  if (d == 64) launch<64>(p, B, stream); else launch<128>(p, B, stream);
   return true;
-}
-
-void paged_decode_join(const PagedDecode& p, const PagedJoin& join, int B, int d, cudaStream_t stream) {
-  if (d == 64) launch<64, true>(p, join, B, stream); else launch<128, true>(p, join, B, stream);
-  count_launch();
 }
 
 }  // namespace tk

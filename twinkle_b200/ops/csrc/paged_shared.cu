@@ -4,11 +4,12 @@
 // instead of 2·G per sequence, read n times.  Up to a few hundred rows the keys and values (4·D bytes per token and key head, once per group) are what
 // bounds it, so the work is laid out to stream them: an item is up to 128 query rows of one group and a run of 128-token blocks of its prefix, a CTA takes an
 // item for one key head, and the items are cut so that they fill the SMs evenly (`ops.shared_prefix`).  Each writes its rows' running maximum, sum and unscaled
-// output in fp32; the decode kernel that reads every sequence's own pages (paged_decode.cu) joins them with what it found itself.
+// output in fp32.  A second kernel for the sequences' own pages runs beside this one on the same SMs and does likewise; a third joins what both found.
 //
 // In a CTA the blocks of its run alternate between two streams of their own scores and output in tensor memory, so that the products of one run under
-// the softmax of the other; both meet the same query rows and are joined at the end.  Pages are loaded as boxes of up to 128 rows of a page (any page size that is a multiple of 8).
-// Tensor memory: scores [0,128) and [128,256), P in place of its scores, output [256,384) and [384,512).
+// the softmax of the other; both meet the same query rows and are joined at the end.  Pages are loaded as boxes of up to 128 whole rows of a page (any page size that is a multiple
+// of 8): in shared memory eight rows' first 128 bytes lie together, then the same rows' second 128 bytes, then the next eight rows.
+// Tensor memory: scores [0,128) and [128,256), both parts of P in place of their scores (32 at a time), output [256,384) and [384,512).
 //
 // Precision: probabilities go into the product as two bf16 parts, the leading one cut off (not rounded), so that neither part is negative and an infinite
 // value comes out as infinity; their sum is within 2^-16 of the value.  The second product costs nothing while memory is the bound.
@@ -19,22 +20,21 @@
 #include "common.cuh"
 #include "elect.cuh"
 #include "host.h"
-#include "paged_decode.h"
+#include "mma16.cuh"
 
 namespace tk {
 
 using bf16 = __nv_bfloat16;
 
 namespace sp {
-constexpr int ROWS = 128, BKV = 128, THREADS = 320, ITEM = 8;
+constexpr int ROWS = 128, BKV = 128, THREADS = 352, ITEM = 8, JOIN_WARPS = 4;
 constexpr int ATOM_BYTES = 128 * 64 * 2;
 constexpr float RESCALE_THRESHOLD = 8.f;      // log2 units
 template <int D>
 struct Smem {
-  static constexpr int TILE = D / 64 * ATOM_BYTES, STAGES = D == 128 ? 3 : 4;
-  static constexpr int Q = 0, K = TILE, V = K + STAGES * TILE, BAR = V + STAGES * TILE, STAT = BAR + 256, TOTAL = STAT + 2 * ROWS * 4 + 1024;
-  static constexpr int PITCH = D + 4;         // of the exchanged output, in floats: rows on different banks
-  static_assert(ROWS * PITCH * 4 <= STAGES * TILE, "the exchange goes where the keys were");
+  static constexpr int TILE = D / 64 * ATOM_BYTES, STAGES = D == 128 ? 2 : 4;
+  static constexpr int Q = 0, K = TILE, V = K + STAGES * TILE, BAR = V + STAGES * TILE, TOTAL = BAR + 256 + 1024;
+  static_assert(ROWS * D * 4 <= STAGES * TILE, "the exchange goes where the keys were");
   static_assert(TOTAL <= 232448, "shared memory of a CTA");
 };
 }  // namespace sp
@@ -42,7 +42,7 @@ struct Smem {
 struct SharedPrefix {
   const int* items;        // [items][8]: first sequence, sequences, first block of 128 tokens, blocks, tokens of the prefix, slot
   const int* tables;
-  float* part;             // [slots, hkv, 128, D]
+  float* part;             // [slots, hkv, 128, D], four columns c of row r at c ^ (r & 7)
   float2* stat;            // [slots, hkv, 128] maximum (log2 units), sum
   int max_blocks, block_size, box, num_blocks, hkv, G, sequences, slots;
   float scale_log2;
@@ -101,56 +101,53 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   tc_fence_after();
   const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
 
-  if (warp == 8) {
-    // ------------------------------------------------------------- producer
-    // Lane = one box of a block's keys and of its values (at most 16 boxes of rows times two chunks of columns).  A box past the prefix or outside the pool starts behind the
-    // tensor and arrives as zeros.
-    const int boxes = BKV / p.box, unit = lane % boxes, c = lane / boxes;
-    const bool mine = c < CH;
-    const int outside = p.num_blocks * p.block_size;
-    auto lookup = [&](int j) -> int {
-      const int t = (tile0 + j) * BKV + unit * p.box;
-      if (!mine || j >= n || t >= tokens) return outside;
+  if (warp == 8 || warp == 10) {
+    // ------------------------------------------- producers: warp 8 the query and the keys, warp 10 the values
+    // A block is up to 16 boxes of 8 rows or more of a page.  Lanes look up a box each, 32 ahead of those that are loaded (the table comes from memory as the pages do); the warp
+    // walks the boxes together and one thread issues.  A box past the prefix or outside the pool starts behind the tensor and arrives as zeros.
+    const bool keys = warp == 8;
+    const CUtensorMap* map = keys ? &tmK : &tmV;
+    uint64_t *full = keys ? k_full : v_full, *empty = keys ? k_empty : v_empty;
+    uint8_t* tile = smem + (keys ? S::K : S::V);
+    const int boxes = BKV / p.box, octets = p.box / 8, outside = p.num_blocks * (p.block_size / 8);
+    auto lookup = [&](int box) -> int {
+      const int t = tile0 * BKV + box * p.box;
+      if (box >= n * boxes || t >= tokens) return outside;
       const int block = p.tables[static_cast<size_t>(row0) * p.max_blocks + t / p.block_size];
       if (block < 0 || block >= p.num_blocks) {      // whoever reads the word next raises
         atomicCAS(p.err, 0, ERR_BOUNDS);
         return outside;
       }
-      return block * p.block_size + t % p.block_size;
+      return (block * p.block_size + t % p.block_size) / 8;
     };
-    int row = lookup(0), issued = 0;
-    if (lane == 0) {
-      tma_prefetch_desc(&tmK);
-      tma_prefetch_desc(&tmV);
-      mbar_expect_tx(q_full, CH * (ROWS / p.G) * p.G * 128);
+    int places = lookup(lane), ahead = lookup(32 + lane), j = 0;
+    if (elect_one()) {
+      tma_prefetch_desc(map);
+      if (keys) {
+        mbar_expect_tx(q_full, CH * (ROWS / p.G) * p.G * 128);
 #pragma unroll
-      for (int i = 0; i < CH; ++i) tma_load_3d(smem + S::Q + i * ATOM_BYTES, &tmQ, q_full, i * 64, kvh * p.G, row0);
-    }
-    bool ok = true;
-    for (int j = 0; j < n; ++j) {
-      const int st = j % NS, next = lookup(j + 1);
-      if (j >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&k_empty[st], (j / NS - 1) & 1, p.err, ERR_ATTN_WAIT));
-      if (!ok) break;
-      if (lane == 0) mbar_expect_tx(&k_full[st], S::TILE);
-      __syncwarp();
-      if (mine) tma_load_3d(smem + S::K + st * S::TILE + c * ATOM_BYTES + unit * p.box * 128, &tmK, &k_full[st], c * 64, kvh, row);
-      if (j >= NS) ok = __all_sync(0xffffffffu, mbar_wait(&v_empty[st], (j / NS - 1) & 1, p.err, ERR_ATTN_WAIT));
-      if (!ok) {
-        mbar_wait(&k_full[st], (j / NS) & 1, nullptr, 0);
-        break;
+        for (int i = 0; i < CH; ++i) tma_load_3d(smem + S::Q + i * ATOM_BYTES, &tmQ, q_full, i * 64, kvh * p.G, row0);
       }
-      if (lane == 0) mbar_expect_tx(&v_full[st], S::TILE);
-      __syncwarp();
-      if (mine) tma_load_3d(smem + S::V + st * S::TILE + c * ATOM_BYTES + unit * p.box * 128, &tmV, &v_full[st], c * 64, kvh, row);
-      row = next;
-      issued = j + 1;
     }
-    if (!ok) {       // nobody may leave while copies are on their way into this CTA's memory
-      mbar_wait(q_full, 0, nullptr, 0);
-      for (int j = max(0, issued - NS); j < issued; ++j) {
-        mbar_wait(&k_full[j % NS], (j / NS) & 1, nullptr, 0);
-        mbar_wait(&v_full[j % NS], (j / NS) & 1, nullptr, 0);
+    __syncwarp();
+    for (; j < n; ++j) {
+      const int st = j % NS, from = j * boxes & 31;      // boxes are a power of two: a block's are together
+      if (j > 0 && from == 0) {
+        places = ahead;
+        ahead = lookup(j * boxes + 32 + lane);
       }
+      if (j >= NS && !__all_sync(0xffffffffu, mbar_wait(&empty[st], (j / NS - 1) & 1, p.err, ERR_ATTN_WAIT))) break;
+      if (elect_one()) mbar_expect_tx(&full[st], S::TILE);
+      __syncwarp();
+      for (int u = 0; u < boxes; ++u) {
+        const int octet = __shfl_sync(0xffffffffu, places, from + u);
+        if (elect_one()) tma_load_5d(tile + st * S::TILE + u * octets * CH * 1024, map, &full[st], 0, 0, 0, kvh, octet);
+        __syncwarp();
+      }
+    }
+    if (j < n) {       // gave up: nobody may leave while copies are on their way into this CTA's memory
+      if (keys) mbar_wait(q_full, 0, nullptr, 0);
+      for (int i = max(0, j - NS); i < j; ++i) mbar_wait(&full[i % NS], (i / NS) & 1, nullptr, 0);
     }
   } else if (warp == 9) {
     // ----------------------------------------------------------- MMA issuer
@@ -162,13 +159,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       const int st = j % NS, t = j & 1;
       if (!wait(&k_full[st], (j / NS) & 1)) return false;
       tc_fence_after();
-      const uint64_t dk = umma_desc(smem_u32(smem + S::K + st * S::TILE), 16, 1024);
+      const uint64_t dk = umma_desc(smem_u32(smem + S::K + st * S::TILE), 16, CH * 1024);
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < CH * 4; ++k) {
-          const uint32_t off = ((k >> 2) * ATOM_BYTES + (k & 3) * 32) >> 4;
-          umma_bf16(tmem_base + t * 128, dq + off, dk + off, idesc_s, k ? 1u : 0u);
-        }
+        for (int k = 0; k < CH * 4; ++k)
+          umma_bf16(tmem_base + t * 128, dq + (((k >> 2) * ATOM_BYTES + (k & 3) * 32) >> 4), dk + (((k >> 2) * 1024 + (k & 3) * 32) >> 4), idesc_s, k ? 1u : 0u);
         umma_commit(&s_full[t]);
         umma_commit(&k_empty[st]);
       }
@@ -181,13 +176,13 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       ok = wait(&v_full[st], (j / NS) & 1) && wait(&p_ready[t], (j >> 1) & 1);
       if (!ok) break;
       tc_fence_after();
-      const uint64_t dv = umma_desc(smem_u32(smem + S::V + st * S::TILE), ATOM_BYTES, 1024);
+      const uint64_t dv = umma_desc(smem_u32(smem + S::V + st * S::TILE), 1024, CH * 1024);
       if (elect_one()) {
 #pragma unroll
         for (int part = 0; part < 2; ++part)
 #pragma unroll
           for (int k = 0; k < BKV / 16; ++k)
-            umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + part * 64 + k * 8, dv + k * (2048 >> 4), idesc_o, part + k > 0 ? 1u : static_cast<uint32_t>(j > 1));
+            umma_bf16_ts(tmem_base + 256 + t * 128, tmem_base + t * 128 + (k >> 1) * 32 + part * 16 + (k & 1) * 8, dv + k * (2 * CH * 1024 >> 4), idesc_o, part + k > 0 ? 1u : static_cast<uint32_t>(j > 1));
         umma_commit(&v_empty[st]);
         if (j + 2 >= n) umma_commit(&o_done[t]);
       }
@@ -196,7 +191,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     }
   } else {
     // -------------------------------------------------------------- softmax
-    const int t = warp >> 2, row = (warp & 3) * 32 + lane;
+    // Warps whose rows no sequence has only keep the products going: what their rows of the output hold is not stored.
+    const int t = warp >> 2, row = (warp & 3) * 32 + lane, live = seqs * p.G;
+    const bool idle = (warp & 3) * 32 >= live;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t ts = tmem_base + t * 128 + lane_off, to = tmem_base + 256 + t * 128 + lane_off;
     const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
@@ -205,32 +202,29 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     bool dead = false;
     for (int j = t; j < n; j += 2) {
       if (!mbar_wait(&s_full[t], (j >> 1) & 1, p.err, ERR_ATTN_WAIT)) { dead = true; break; }
+      if (idle) {
+        mbar_arrive(&p_ready[t]);
+        continue;
+      }
       tc_fence_after();
-      float sc[128];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) tmem_ld32(ts + c * 32, *reinterpret_cast<uint32_t(*)[32]>(sc + c * 32));
-      tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 128; i += 2) {
-        const float2 x = mul2(make_float2(sc[i], sc[i + 1]), scale2);
-        sc[i] = x.x;
-        sc[i + 1] = x.y;
-      }
+      // Scores are read twice and a few columns at a time: the code of a block that keeps them in registers is 10 KB, and its first run then waits for every line of it.
       const int left = tokens - (tile0 + j) * BKV;
-      if (left < BKV) {
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll 1
+      for (int c = 0; c < 4; c += 2) {
+        uint32_t r[2][32];
+        tmem_ld32(ts + c * 32, r[0]);
+        tmem_ld32(ts + c * 32 + 32, r[1]);
+        tmem_ld_wait();
+        if (left < BKV) {
 #pragma unroll
-        for (int i = 0; i < 128; ++i)
-          if (i >= left) sc[i] = -INFINITY;
-      }
-      float mx4[4] = {sc[0], sc[1], sc[2], sc[3]};
+          for (int i = 0; i < 64; ++i)
+            if (c * 32 + i >= left) r[i >> 5][i & 31] = 0xff800000u;      // −∞
+        }
 #pragma unroll
-      for (int i = 4; i < 128; i += 4) {
-        mx4[0] = fmaxf(mx4[0], sc[i]);
-        mx4[1] = fmaxf(mx4[1], sc[i + 1]);
-        mx4[2] = fmaxf(mx4[2], sc[i + 2]);
-        mx4[3] = fmaxf(mx4[3], sc[i + 3]);
+        for (int i = 0; i < 64; ++i) mx4[i & 3] = fmaxf(mx4[i & 3], __uint_as_float(r[i >> 5][i & 31]));
       }
-      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
+      const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * p.scale_log2;      // the scale is positive
       float alpha = 1.f;
       bool rescale = false;
       if (mx > m + RESCALE_THRESHOLD || (m == -INFINITY && mx != -INFINITY)) {
@@ -253,73 +247,89 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         tmem_st_wait();
       }
-      const float2 neg = make_float2(-sub, -sub);
+      const float2 neg = make_float2(-sub, -sub), tiny = make_float2(1.17549435e-38f, 1.17549435e-38f);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {         // 32 scores become 16 columns of leading parts and 16 of what is left
+        uint32_t r[32];
+        tmem_ld32(ts + c * 32, r);
+        tmem_ld_wait();
+        if (left < BKV) {
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint32_t lead[32], rest[32];
+          for (int i = 0; i < 32; ++i)
+            if (c * 32 + i >= left) r[i] = 0xff800000u;
+        }
+        uint32_t parts[32];
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-          const float2 x = add2(make_float2(sc[half * 64 + 2 * i], sc[half * 64 + 2 * i + 1]), neg);
+        for (int i = 0; i < 16; ++i) {
+          const float2 x = fma2(make_float2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), scale2, neg);
           const float2 e = make_float2(fast_exp2(x.x), fast_exp2(x.y));
           l2 = add2(l2, e);
           const uint32_t a = __float_as_uint(e.x), b = __float_as_uint(e.y);
-          lead[i] = __byte_perm(a, b, 0x7632);
-          // what was cut off, and at least 2^-126: an infinite value then adds to an infinite sum
-          rest[i] = pack_bf16(fmaxf(e.x - __uint_as_float(a & 0xffff0000u), 1.17549435e-38f), fmaxf(e.y - __uint_as_float(b & 0xffff0000u), 1.17549435e-38f));
+          parts[i] = __byte_perm(a, b, 0x7632);
+          // what was cut off, and never nothing: an infinite value then adds to an infinite sum
+          const float2 cut = add2(add2(e, make_float2(__uint_as_float((a & 0xffff0000u) ^ 0x80000000u), __uint_as_float((b & 0xffff0000u) ^ 0x80000000u))), tiny);
+          parts[16 + i] = pack_bf16(cut.x, cut.y);
         }
-        tmem_st32(ts + half * 32, lead);
-        tmem_st32(ts + 64 + half * 32, rest);
+        tmem_st32(ts + c * 32, parts);
       }
       tmem_st_wait();
       tc_fence_before();
       mbar_arrive(&p_ready[t]);
     }
     // ------------------------------------------------------------- epilogue
-    // The second stream hands its rows over in shared memory, which no copy or product uses any more; the first writes the sum of both.
+    // Each stream hands the other half of its columns over in shared memory, which no copy or product uses any more, and sums the half that it gets, in place; the
+    // rows then leave in one copy.  Four columns of row r lie at place c ^ (r & 7), there and in the result: threads with a row each meet all banks.
     float* xo = reinterpret_cast<float*>(smem + S::K);
-    float* xs = reinterpret_cast<float*>(smem + S::STAT);
+    float* xs = reinterpret_cast<float*>(smem + S::Q);
     const bool two = n > 1;
     dead = dead || !mbar_wait(&o_done[0], 0, p.err, ERR_ATTN_WAIT) || (two && !mbar_wait(&o_done[1], 0, p.err, ERR_ATTN_WAIT));
     tc_fence_after();
-    float l = l2.x + l2.y;
-    if (t == 1 && two && !dead) {
-      xs[row] = m;
-      xs[ROWS + row] = l;
+    const float l = l2.x + l2.y;
+    auto place = [&](int c) { return reinterpret_cast<float4*>(xo + row * D + ((c ^ (row & 7)) << 2)); };
+    xs[t * 2 * ROWS + row] = m;
+    xs[(t * 2 + 1) * ROWS + row] = l;
+    if (two && !dead) {
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < D / 64; ++c) {
+        const int col = (t ^ 1) * (D / 2) + c * 32;
         uint32_t r[32];
-        tmem_ld32(to + c * 32, r);
+        tmem_ld32(to + col, r);
         tmem_ld_wait();
 #pragma unroll
         for (int i = 0; i < 32; i += 4)
-          *reinterpret_cast<float4*>(xo + row * S::PITCH + c * 32 + i) =
-              make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
+          *place((col + i) >> 2) = make_float4(__uint_as_float(r[i]), __uint_as_float(r[i + 1]), __uint_as_float(r[i + 2]), __uint_as_float(r[i + 3]));
       }
     }
     asm volatile("bar.sync 1, 256;" ::: "memory");
-    if (t == 0 && !dead) {
-      const float m1 = two ? xs[row] : -INFINITY, l1 = two ? xs[ROWS + row] : 0.f, mm = fmaxf(m, m1);
-      const float a0 = m == -INFINITY ? 0.f : fast_exp2(m - mm), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - mm);
-      const bool live = row < seqs * p.G;
-      const size_t at = (static_cast<size_t>(slot) * p.hkv + kvh) * ROWS + row;
-      if (live) p.stat[at] = make_float2(mm, l * a0 + l1 * a1);
+    const size_t at = (static_cast<size_t>(slot) * p.hkv + kvh) * ROWS;
+    if (!dead) {
+      const float m0 = xs[row], l0 = xs[ROWS + row], m1 = two ? xs[2 * ROWS + row] : -INFINITY, l1 = two ? xs[3 * ROWS + row] : 0.f, mm = fmaxf(m0, m1);
+      const float a0 = m0 == -INFINITY ? 0.f : fast_exp2(m0 - mm), a1 = m1 == -INFINITY ? 0.f : fast_exp2(m1 - mm);
+      const float mine = t == 0 ? a0 : a1, theirs = t == 0 ? a1 : a0;
+      if (t == 0 && row < live) p.stat[at + row] = make_float2(mm, l0 * a0 + l1 * a1);
 #pragma unroll 1
-      for (int c = 0; c < D / 32; ++c) {
+      for (int c = 0; c < D / 64; ++c) {
+        const int col = t * (D / 2) + c * 32;
+        // without a second stream its half of the columns comes from the first
         uint32_t r[32];
-        tmem_ld32(to + c * 32, r);
+        tmem_ld32((two ? to : tmem_base + 256 + lane_off) + col, r);
         tmem_ld_wait();
-        if (live) {
 #pragma unroll
-          for (int i = 0; i < 32; i += 4) {
-            float4 o = make_float4(__uint_as_float(r[i]) * a0, __uint_as_float(r[i + 1]) * a0, __uint_as_float(r[i + 2]) * a0, __uint_as_float(r[i + 3]) * a0);
-            if (two) {
-              const float4 x = *reinterpret_cast<const float4*>(xo + row * S::PITCH + c * 32 + i);
-              o = make_float4(fmaf(x.x, a1, o.x), fmaf(x.y, a1, o.y), fmaf(x.z, a1, o.z), fmaf(x.w, a1, o.w));
-            }
-            *reinterpret_cast<float4*>(p.part + at * D + c * 32 + i) = o;
-          }
+        for (int i = 0; i < 32; i += 4) {
+          const float s = two ? mine : a0;
+          float4 o = make_float4(__uint_as_float(r[i]) * s, __uint_as_float(r[i + 1]) * s, __uint_as_float(r[i + 2]) * s, __uint_as_float(r[i + 3]) * s);
+          float4* x = place((col + i) >> 2);
+          if (two) o = make_float4(fmaf(x->x, theirs, o.x), fmaf(x->y, theirs, o.y), fmaf(x->z, theirs, o.z), fmaf(x->w, theirs, o.w));
+          *x = o;
         }
       }
+    }
+    fence_proxy_async();
+    asm volatile("bar.sync 1, 256;" ::: "memory");
+    if (threadIdx.x == 0 && !dead) {
+      asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(p.part + at * D), "r"(smem_u32(xo)), "r"(live * D * 4) : "memory");
+      asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+      asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");      // the rest is over when the kernel is
     }
   }
   tc_fence_before();
@@ -330,18 +340,309 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   }
 }
 
+// A sequence has a part in its group's prefix when it is as long (`r`: its line of the plan); else it attends to all of its own keys.
+__device__ __forceinline__ bool has_prefix(const int4& r, int n, int slots, int group) {
+  return n >= r.x && r.x >= 0 && r.z > 0 && r.y >= 0 && r.y + r.z <= slots && r.w >= 0 && r.w + group <= sp::ROWS;
+}
+// The sequences' own pages: a CTA per run of 16 tiles of 16 tokens or more of a sequence, key head and eight query heads; tiles go round robin over its four warps, each with rings of
+// two tiles of keys and two of values filled by cp.async.  Products as in paged_decode.cu: heads are rows 0–7, rows 8–15 take what rounding the probabilities left.  Its CTAs fit an SM
+// beside one of the prefix kernel's (shared memory, and 200 registers a thread: 3 warps of the other on a scheduler leave no more), so that both stream from memory at once.
+namespace ow {
+constexpr int WARPS = 4, TILE = 16, RUN = 16, RUNS = 8, HEADS = 8;
+template <int D> constexpr int half_bytes() { return 2 * TILE * D; }            // a tile's keys or values
+template <int D> constexpr int smem_bytes() { return WARPS * 4 * half_bytes<D>(); }
+}  // namespace ow
+// Tiles of 16 tokens that hold the keys first … n of a sequence, and how many of them make a run when there are `runs` CTAs for it
+__device__ __forceinline__ int own_tiles(int first, int n) { return n > (first & ~15) ? (n - (first & ~15) + 15) / 16 : 0; }
+__device__ __forceinline__ int run_tiles(int tiles, int runs) { return max(ow::RUN, (tiles + runs - 1) / runs); }
+
+struct OwnPages {
+  const bf16 *q, *kc, *vc;
+  const int *tables, *seq_lens, *rows;
+  float* part;             // [runs, B, hq, D] unscaled outputs; a run without tokens writes nothing
+  float2* stat;            // [runs, B, hq] maximum (log2 units), sum
+  int B, hq, hkv, G, block_size, max_blocks, num_blocks, slots, runs;
+  float scale_log2;
+  int* err;
+};
+
+template <int D>
+__global__ void __launch_bounds__(ow::WARPS * 32, 3) own_pages_kernel(const OwnPages p) {
+  using namespace ow;
+  constexpr int CH = D / 8, RPI = 32 / CH, ROW = 2 * D;      // 16-byte chunks of a row, rows that one load of a warp covers, bytes of a row
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  // one CTA sees the prefix kernel end, so that this kernel ends after it
+  auto leave = [] {
+    if (blockIdx.x == 0 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+  };
+  const int groups = (p.G + HEADS - 1) / HEADS, kvh = blockIdx.y / groups, g0 = blockIdx.y % groups * HEADS, h0 = kvh * p.G + g0, GH = min(HEADS, p.G - g0), b = blockIdx.z, run = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, hrow = lane >> 2;
+  const int4 line = reinterpret_cast<const int4*>(p.rows)[b];
+  const int n = min(p.seq_lens[b], p.max_blocks * p.block_size), first = has_prefix(line, n, p.slots, p.G) ? line.x : 0;
+  const int total = own_tiles(first, n), per = run_tiles(total, p.runs), tiles = min(per, total - run * per);
+  if (tiles <= 0) return leave();
+  const int base = (first & ~(TILE - 1)) + run * per * TILE, mine = (tiles - warp + WARPS - 1) / WARPS;
+
+  extern __shared__ __align__(128) uint8_t smem[];
+  uint8_t *kring = smem + warp * 4 * half_bytes<D>(), *vring = kring + 2 * half_bytes<D>();
+  const int* table = p.tables + static_cast<size_t>(b) * p.max_blocks;
+  // row of the pools that holds token (lane & 15) of this warp's tile i, or −1
+  auto lookup = [&](int i) -> int {
+    const int t = base + (warp + i * WARPS) * TILE + (lane & 15);
+    if (i >= mine || t >= n || t < first) return -1;
+    const int block = table[t / p.block_size];
+    if (block < 0 || block >= p.num_blocks) {      // whoever reads the word next raises
+      atomicCAS(p.err, 0, ERR_BOUNDS);
+      return -1;
+    }
+    return block * p.block_size + t % p.block_size;
+  };
+  // keys or values of a tile; chunks of a row are exchanged so that ldmatrix meets all banks
+  auto fetch = [&](const bf16* pool, uint8_t* to, bool live, int rows) {
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < TILE / RPI; ++k) {
+        const int r = k * RPI + lane / CH, c = lane % CH, row = __shfl_sync(0xffffffffu, rows, r);
+        cp_async16(smem_u32(to) + r * ROW + ((c ^ (r & 7)) << 4), pool + (static_cast<size_t>(max(row, 0)) * p.hkv + kvh) * D + c * 8, row >= 0);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int rows[2] = {lookup(0), lookup(1)}, ahead = lookup(2);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    fetch(p.kc, kring + i * half_bytes<D>(), i < mine, rows[i]);
+    fetch(p.vc, vring + i * half_bytes<D>(), i < mine, rows[i]);
+  }
+  // the heads' rows of A; rows 8–15 are zero for the scores
+  uint32_t qa[D / 16][2];
+#pragma unroll
+  for (int k = 0; k < D / 16; ++k) {
+    qa[k][0] = qa[k][1] = 0u;
+    if (hrow < GH) {
+      const uint32_t* q = reinterpret_cast<const uint32_t*>(p.q + (static_cast<size_t>(b) * p.hq + h0 + hrow) * D + k * 16 + quad * 2);
+      qa[k][0] = q[0];
+      qa[k][1] = q[4];
+    }
+  }
+  float m = -INFINITY, l = 0.f, acc[D / 8][4];
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+  for (int i = 0; i < mine; ++i) {
+    uint8_t *ks = kring + (i & 1) * half_bytes<D>(), *vs = vring + (i & 1) * half_bytes<D>();
+    asm volatile("cp.async.wait_group 3;" ::: "memory");
+    __syncwarp();
+    float s[2][4] = {};
+    {
+      const int r = (lane & 7) + ((lane >> 4) << 3), half = (lane >> 3) & 1;      // tokens 0–7 chunks 0, 1; tokens 8–15 chunks 0, 1
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        uint32_t bk[4];
+        ldsm4(bk, reinterpret_cast<const bf16*>(ks + r * ROW + (((2 * k + half) ^ (r & 7)) << 4)));
+        const uint32_t a[4] = {qa[k][0], 0u, qa[k][1], 0u};
+        mma(s[0], a, bk[0], bk[1]);
+        mma(s[1], a, bk[2], bk[3]);
+      }
+    }
+    __syncwarp();
+    const int places = ahead;               // of the tile after the next, into the places that this one leaves
+    ahead = lookup(i + 3);
+    fetch(p.kc, ks, i + 2 < mine, places);
+    const int t0 = base + (warp + i * WARPS) * TILE + quad * 2;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int t = t0 + j * 8 + e;
+        s[j][e] = t < n && t >= first ? s[j][e] * p.scale_log2 : -INFINITY;
+        mx = fmaxf(mx, s[j][e]);
+      }
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    const float mn = fmaxf(m, mx), sub = mn == -INFINITY ? 0.f : mn;
+    if (__any_sync(0xffffffffu, mn != m)) {
+      const float corr = fast_exp2(m - sub);       // 2^−∞ = 0 before the first key
+      l *= corr;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[j][e] *= corr;
+    }
+    m = mn;
+    uint32_t a[4];                                  // leading parts in rows 0–7, remainders in rows 8–15
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      const float p0 = fast_exp2(s[j][0] - sub), p1 = fast_exp2(s[j][1] - sub);
+      l += p0 + p1;
+      split2(p0, p1, a[2 * j], a[2 * j + 1]);
+    }
+    asm volatile("cp.async.wait_group 3;" ::: "memory");
+    __syncwarp();
+    const int r = lane & 15, half = lane >> 4;     // tokens 0–15 of chunk 2j, tokens 0–15 of chunk 2j + 1
+#pragma unroll
+    for (int j = 0; j < D / 16; ++j) {
+      uint32_t bv[4];
+      ldsm4t(bv, reinterpret_cast<const bf16*>(vs + r * ROW + (((2 * j + half) ^ (r & 7)) << 4)));
+      mma(acc[2 * j], a, bv[0], bv[1]);
+      mma(acc[2 * j + 1], a, bv[2], bv[3]);
+    }
+    __syncwarp();
+    fetch(p.vc, vs, i + 2 < mine, places);
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  __syncthreads();                                  // the rings are free: they take the merge
+  float* part = reinterpret_cast<float*>(smem);                       // [WARPS][HEADS][D]
+  float* stat = part + WARPS * HEADS * D;                             // [2][WARPS][HEADS] maximum, sum
+#pragma unroll
+  for (int j = 0; j < D / 8; ++j)
+    *reinterpret_cast<float2*>(&part[(warp * HEADS + hrow) * D + j * 8 + quad * 2]) = make_float2(whole(acc[j][0], acc[j][2]), whole(acc[j][1], acc[j][3]));
+  if (quad == 0) {
+    stat[warp * HEADS + hrow] = m;
+    stat[(WARPS + warp) * HEADS + hrow] = l;
+  }
+  __syncthreads();
+  const size_t at = (static_cast<size_t>(run) * p.B + b) * p.hq + h0;
+  for (int i = threadIdx.x; i < GH * D; i += WARPS * 32) {
+    const int h = i / D;
+    float mm = stat[h];
+#pragma unroll
+    for (int w = 1; w < WARPS; ++w) mm = fmaxf(mm, stat[w * HEADS + h]);
+    float o = 0.f, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float mw = stat[w * HEADS + h], c = mw == -INFINITY ? 0.f : fast_exp2(mw - mm);
+      o += part[w * HEADS * D + i] * c;
+      ll += stat[(WARPS + w) * HEADS + h] * c;
+    }
+    p.part[at * D + i] = o;
+    if (i % D == 0) p.stat[at + h] = make_float2(mm, ll);
+  }
+  leave();
+}
+
+// Joins what the pieces of a prefix and a sequence's own pages found: W warps per query head, each with its share of both.
+struct SharedJoin {
+  const int *rows, *seq_lens;
+  const float *part, *own_part;
+  const float2 *stat, *own_stat;
+  bf16* out;
+  int total, hq, hkv, G, slots, runs, width;      // width: tokens that a row of the table has room for
+};
+
+template <int D, int W>
+__global__ void __launch_bounds__(sp::JOIN_WARPS * 32) shared_join_kernel(const SharedJoin p) {
+  constexpr int E = D / 32, HEADS = sp::JOIN_WARPS / W;      // elements of a lane, heads of a CTA
+  __shared__ float s_acc[W > 1 ? W : 1][D + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, part = warp % W, at = blockIdx.x * HEADS + warp / W;
+  if (at >= p.total) return;                  // of one head per CTA all warps leave or none
+  const int b = at / p.hq, h = at - b * p.hq, kvh = h / p.G;
+  const int4 r = reinterpret_cast<const int4*>(p.rows)[b];      // older than the kernels before this one
+  const int n = min(p.seq_lens[b], p.width), slots = has_prefix(r, n, p.slots, p.G) ? r.z : 0, row = r.w + h - kvh * p.G;
+  const int own_total = own_tiles(slots > 0 ? r.x : 0, n), per = run_tiles(own_total, p.runs), owns = (own_total + per - 1) / per;
+  const size_t found = (static_cast<size_t>(r.y) * p.hkv + kvh) * sp::ROWS + row, next = static_cast<size_t>(p.hkv) * sp::ROWS;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // its own runs: lane k holds the k-th
+  const float2 own = lane < owns ? p.own_stat[lane * static_cast<size_t>(p.total) + at] : make_float2(-INFINITY, 0.f);
+  float m = own.x;
+  for (int k = lane; k < slots; k += 32) m = fmaxf(m, p.stat[found + k * next].x);
+  m = warp_max(m);
+  float acc[E], l = 0.f;
+#pragma unroll
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  auto add = [&](const float* from, float w) {
+    float v[E];
+    if constexpr (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
+    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(from);
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], w, acc[e]);
+  };
+  const int c = lane * E, mine = (slots - part + W - 1) / W;      // this warp's pieces: part, part + W, …
+  const float* from = p.part + (found + part * next) * D + ((c >> 2 ^ (row & 7)) << 2 | (c & 3));
+  for (int k0 = 0; k0 < mine; k0 += 32) {
+    const float2 s = k0 + lane < mine ? p.stat[found + (part + (k0 + lane) * W) * next] : make_float2(-INFINITY, 0.f);
+    const float w = s.x == -INFINITY ? 0.f : fast_exp2(s.x - m);
+    l += s.y * w;
+#pragma unroll 8
+    for (int k = 0; k < min(32, mine - k0); ++k) add(from + (k0 + k) * W * next * D, __shfl_sync(0xffffffffu, w, k));
+  }
+  const float w = own.x == -INFINITY ? 0.f : fast_exp2(own.x - m);
+  if (part == 0) l += own.y * w;
+  l = warp_sum(l);
+#pragma unroll 4
+  for (int k = part; k < owns; k += W) add(p.own_part + (k * static_cast<size_t>(p.total) + at) * D + c, __shfl_sync(0xffffffffu, w, k));
+  if constexpr (W > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_acc[part][c + e] = acc[e];
+    if (lane == 0) s_acc[part][D] = l;
+    __syncthreads();
+    if (part > 0) return;
+    for (int i = 1; i < W; ++i) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] += s_acc[i][c + e];
+      l += s_acc[i][D];
+    }
+  }
+  const float scale = l > 0.f ? 1.f / l : l;         // a sum that is not a number stays one
+  uint32_t o[E / 2];
+#pragma unroll
+  for (int e = 0; e < E; e += 2) o[e / 2] = pack_bf16(l == 0.f ? 0.f : acc[e] * scale, l == 0.f ? 0.f : acc[e + 1] * scale);
+  bf16* to = p.out + static_cast<size_t>(at) * D + c;
+  if constexpr (E == 4) *reinterpret_cast<uint2*>(to) = make_uint2(o[0], o[1]);
+  else *reinterpret_cast<uint32_t*>(to) = o[0];
+}
+
 template <int D>
 static void launch_prefix(const SharedPrefix& p, int64_t items, const CUtensorMap& tq, const CUtensorMap& tk_, const CUtensorMap& tv, cudaStream_t stream) {
   static OncePerDevice limit;
-  limit(current_device(), [] { TK_CUDA_CHECK(cudaFuncSetAttribute(shared_prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, sp::Smem<D>::TOTAL)); });
+  limit(current_device(), [] {
+    TK_CUDA_CHECK(cudaFuncSetAttribute(shared_prefix_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, sp::Smem<D>::TOTAL));
+    // an SM that gives this kernel no more than it asks for has no room for the next one's CTAs until it is idle
+    TK_CUDA_CHECK(cudaFuncSetAttribute(shared_prefix_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  });
   shared_prefix_kernel<D><<<dim3(items, p.hkv), sp::THREADS, sp::Smem<D>::TOTAL, stream>>>(tq, tk_, tv, p);
   count_launch();
   TK_CUDA_CHECK(cudaGetLastError());
 }
 
-// One query token per sequence; plan int32 [items · 8 + B · 4]: the items, then for every sequence the tokens of its prefix, its first slot, its slots and its row in them.
+// A launch that begins while the one before it on the stream runs
+template <typename F, typename P>
+static void launch_beside(F kernel, dim3 ctas, int threads, int smem, const P& p, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = ctas;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  TK_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
+  count_launch();
+}
+
+template <int D>
+static void launch_own(const OwnPages& p, cudaStream_t stream) {
+  static OncePerDevice limit;
+  limit(current_device(), [] {
+    TK_CUDA_CHECK(cudaFuncSetAttribute(own_pages_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ow::smem_bytes<D>()));
+    TK_CUDA_CHECK(cudaFuncSetAttribute(own_pages_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  });
+  launch_beside(own_pages_kernel<D>, dim3(p.runs, p.hkv * ((p.G + ow::HEADS - 1) / ow::HEADS), p.B), ow::WARPS * 32, ow::smem_bytes<D>(), p, stream);
+}
+
+template <int D, int W>
+static void launch_join(const SharedJoin& p, cudaStream_t stream) {
+  constexpr int HEADS = sp::JOIN_WARPS / W;
+  launch_beside(shared_join_kernel<D, W>, dim3((p.total + HEADS - 1) / HEADS), sp::JOIN_WARPS * 32, 0, p, stream);
+}
+
+// One query token per sequence; pieces: slots of a sequence at most; room: tokens that most sequences have at most beside their prefix (what their split is chosen by); plan int32 [items · 8 + B · 4]: the items, then for every sequence the tokens of its prefix, its first slot, its slots and its row in them.
 torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& vc, const torch::Tensor& tables, const torch::Tensor& seq_lens, const torch::Tensor& plan,
-                                int64_t items, int64_t slots, double scale) {
+                                int64_t items, int64_t slots, int64_t pieces, int64_t room, double scale) {
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kBFloat16 && q.is_contiguous() && q.dim() == 3, "q [B,Hq,D] bf16");
   TORCH_CHECK(kc.is_contiguous() && vc.is_contiguous() && kc.dim() == 4 && kc.sizes() == vc.sizes() && kc.scalar_type() == torch::kBFloat16 && vc.scalar_type() == torch::kBFloat16,
               "caches [blocks,bs,Hkv,D] bf16 of one shape");
@@ -351,7 +652,7 @@ torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc,
   for (const auto* t : {&q, &kc, &vc}) TORCH_CHECK(t->device() == q.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "q and caches on one device and on 16-byte boundaries");
   for (const auto* t : {&tables, &seq_lens, &plan}) TORCH_CHECK(t->device() == q.device() && t->scalar_type() == torch::kInt32 && t->is_contiguous(), "int32 tables, lengths and plan on the device of q");
   TORCH_CHECK(tables.dim() == 2 && tables.size(0) == B && seq_lens.numel() == B, "a row of the table and a length per sequence");
-  TORCH_CHECK(items > 0 && slots > 0 && plan.numel() == items * sp::ITEM + B * 4, "plan of other sequences");
+  TORCH_CHECK(items > 0 && slots > 0 && room >= 0 && plan.numel() == items * sp::ITEM + B * 4, "plan of other sequences");
   TORCH_CHECK(reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0 && tables.size(1) * bs < (int64_t(1) << 31), "plan on a 16-byte boundary, contexts below 2^31");
   c10::cuda::CUDAGuard guard(q.device());
   auto out = torch::empty_like(q);
@@ -359,17 +660,33 @@ torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc,
   auto part = torch::empty({slots, hkv, sp::ROWS, D}, f32), stat = torch::empty({slots, hkv, sp::ROWS, 2}, f32);
   const int64_t box = std::min<int64_t>(bs & -bs, sp::BKV);      // the largest power of two that divides a page
   const CUtensorMap tq = make_tmap_3d(q.data_ptr(), D, hq, B, D, hq * D, 64, G, sp::ROWS / G);
-  const CUtensorMap tk_ = make_tmap_3d(kc.data_ptr(), D, hkv, kc.size(0) * bs, D, hkv * D, 64, 1, box), tv = make_tmap_3d(vc.data_ptr(), D, hkv, kc.size(0) * bs, D, hkv * D, 64, 1, box);
+  const uint64_t dims[5] = {64, 8, static_cast<uint64_t>(D / 64), static_cast<uint64_t>(hkv), static_cast<uint64_t>(kc.size(0) * bs / 8)};
+  const uint64_t strides[4] = {static_cast<uint64_t>(hkv * D), 64, static_cast<uint64_t>(D), static_cast<uint64_t>(8 * hkv * D)};
+  const uint32_t boxes[5] = {64, 8, static_cast<uint32_t>(D / 64), 1, static_cast<uint32_t>(box / 8)};
+  const CUtensorMap tk_ = make_tmap_5d(kc.data_ptr(), dims, strides, boxes), tv = make_tmap_5d(vc.data_ptr(), dims, strides, boxes);
   SharedPrefix p{};
   p.items = plan.data_ptr<int>(); p.tables = tables.data_ptr<int>(); p.part = part.data_ptr<float>(); p.stat = reinterpret_cast<float2*>(stat.data_ptr<float>());
   p.max_blocks = tables.size(1); p.block_size = bs; p.box = box; p.num_blocks = kc.size(0); p.hkv = hkv; p.G = G; p.sequences = B; p.slots = slots;
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634); p.err = error_word();
   auto stream = at::cuda::getCurrentCUDAStream();
   if (D == 128) launch_prefix<128>(p, items, tq, tk_, tv, stream); else launch_prefix<64>(p, items, tq, tk_, tv, stream);
-  const PagedDecode d{q.data_ptr(), kc.data_ptr(), vc.data_ptr(), tables.data_ptr<int>(), seq_lens.data_ptr<int>(), out.data_ptr(), nullptr, OutGate{}, static_cast<int>(hq), static_cast<int>(hkv),
-                      static_cast<int>(G), static_cast<int>(bs), static_cast<int>(tables.size(1)), 0, 0, p.scale_log2};
-  const PagedJoin join{plan.data_ptr<int>() + items * sp::ITEM, part.data_ptr<float>(), reinterpret_cast<const float2*>(stat.data_ptr<float>()), static_cast<int>(slots), static_cast<int>(kc.size(0)), p.err};
-  paged_decode_join(d, join, B, D, stream);
+  const int* rows = plan.data_ptr<int>() + items * sp::ITEM;
+  // CTAs of a sequence's own part, by what most have (where there is more a CTA's run is longer): 256 tokens each, more where that makes over 14 CTAs per SM
+  const int64_t wide = B * hkv * ((G + ow::HEADS - 1) / ow::HEADS);
+  int64_t runs = std::max<int64_t>(1, std::min<int64_t>(ow::RUNS, (room + ow::RUN * ow::TILE - 1) / (ow::RUN * ow::TILE)));
+  while (runs > 1 && wide * runs > 14 * num_sms()) runs = (runs + 1) / 2;
+  auto own_part = torch::empty({runs, B, hq, D}, f32), own_stat = torch::empty({runs, B, hq, 2}, f32);
+  const OwnPages own{reinterpret_cast<const bf16*>(q.data_ptr()), reinterpret_cast<const bf16*>(kc.data_ptr()), reinterpret_cast<const bf16*>(vc.data_ptr()), tables.data_ptr<int>(),
+                     seq_lens.data_ptr<int>(), rows, own_part.data_ptr<float>(), reinterpret_cast<float2*>(own_stat.data_ptr<float>()), static_cast<int>(B), static_cast<int>(hq),
+                     static_cast<int>(hkv), static_cast<int>(G), static_cast<int>(bs), static_cast<int>(tables.size(1)), static_cast<int>(kc.size(0)), static_cast<int>(slots), static_cast<int>(runs),
+                     p.scale_log2, p.err};
+  if (D == 128) launch_own<128>(own, stream); else launch_own<64>(own, stream);
+  const SharedJoin join{rows, own.seq_lens, p.part, own.part, p.stat, own.stat, reinterpret_cast<bf16*>(out.data_ptr()), static_cast<int>(B * hq), static_cast<int>(hq), static_cast<int>(hkv),
+                        static_cast<int>(G), static_cast<int>(slots), static_cast<int>(runs), static_cast<int>(tables.size(1) * bs)};
+  // heads with many pieces are summed by four warps: 13 sequences with 37 pieces of 32k tokens 35 -> 31 us; with 5 or fewer one warp does (64 sequences 55 against 57)
+  const bool many = pieces > 8;
+  if (D == 128) many ? launch_join<128, 4>(join, stream) : launch_join<128, 1>(join, stream);
+  else many ? launch_join<64, 4>(join, stream) : launch_join<64, 1>(join, stream);
   return out;
 }
 

@@ -181,6 +181,10 @@ class NativeEngine:
         """``share_prompts``: sequences with the same prompt (the samples of a request, repeated prompts) run through it once, share its full cache
         blocks and read them once per step.  Results then differ by the rounding of other tile shapes and orders of sums."""
         self.model, self.cfg, self.share_prompts = model, cfg, share_prompts
+        # Reading shared pages once takes two more launches: it pays from about 28k keys (times key heads) that are not read again, 12k where a step without it decodes on the vector
+        # kernel (fewer than four query heads per key head).  us per layer, together / apart: 8 sequences of 512 tokens with 32/8 heads 12.1 / 15.2, of 256 11.7 / 8.7;
+        # 4 of 512 with 16/8 heads 12.0 / 16.9, of 128 10.6 / 8.1
+        self.share_from = 12288 if cfg.num_attention_heads < 4 * cfg.num_key_value_heads else 28672
         self._plan: Tuple[Any, Optional[ops.SharedPrefix]] = (None, None)      # of the last step with shared prompts
         self.device = device or next(model.parameters()).device
         self.dtype = next(model.parameters()).dtype
@@ -249,11 +253,13 @@ class NativeEngine:
                 blocks.append(len(s.prompt) // self.cache.block_size if s.origin is not None else 0)
             last = s.origin
         blocks = [b if n > 1 else 0 for n, b in zip(sizes, blocks)]
-        if not any(blocks):
+        heads, kv_heads = self._heads()
+        again = sum((n - 1) * b for n, b in zip(sizes, blocks)) * self.cache.block_size * kv_heads
+        if again == 0 or again < self.share_from:
             return None
         key = (tuple(sizes), tuple(blocks), rows, captured)
         if self._plan[0] != key:
-            fill, (heads, kv_heads) = rows - len(seqs), self._heads()
+            fill = rows - len(seqs)
             self._plan = key, ops.shared_prefix(sizes + [1] * fill, blocks + [0] * fill, self.cache.block_size, heads, kv_heads, self.device,
                                                 ops.prefix_items(rows, kv_heads, self.device) if captured else 0)
         return self._plan[1]
