@@ -911,12 +911,12 @@ def cache_copy(pools, src, dst, tokens=None) -> None:
     pools = [p for p in pools if p is not None]
     if not pools:
         return
-    src, dst, tokens = ([int(x) for x in v] for v in (src, dst, () if tokens is None else tokens))
+    src, dst, tokens = (v if isinstance(v, (list, tuple)) else [int(x) for x in v] for v in (src, dst, () if tokens is None else tokens))
     if len(src) != len(dst) or (tokens and len(tokens) != len(src)):
         raise ValueError('cache_copy: one destination (and number of tokens) per source')
     if not src:
         return
-    if all(_cuda(p) for p in pools):
+    if _cuda(pools[0]):
         return ext().cache_copy(pools, src, dst, tokens)
     ref.cache_copy(pools, src, dst, tokens)
 

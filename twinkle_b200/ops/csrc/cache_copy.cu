@@ -9,7 +9,6 @@
 #include <torch/types.h>
 
 #include <algorithm>
-#include <unordered_set>
 
 #include "common.cuh"
 #include "host.h"
@@ -98,18 +97,21 @@ void cache_copy(const std::vector<torch::Tensor>& pools, const std::vector<int64
     base.push_back(reinterpret_cast<char*>(t.data_ptr()));
     bytes.push_back(per);
   }
-  std::unordered_set<int64_t> read, written;
-  std::vector<int64_t> s, d, n;
+  std::vector<int64_t> s, d, n, read(src), written(dst);
   for (size_t i = 0; i < src.size(); ++i) {
     const int64_t k = tokens.empty() ? 1 : tokens[i];
     TORCH_CHECK(src[i] >= 0 && src[i] < rows && dst[i] >= 0 && dst[i] < rows, "cache_copy: rows ", src[i], " -> ", dst[i], " of ", rows);
     TORCH_CHECK(k >= 0 && k <= row_units, "cache_copy: ", k, " tokens of a row of ", row_units);
-    TORCH_CHECK(written.insert(dst[i]).second, "cache_copy: row ", dst[i], " is written twice");
-    read.insert(src[i]);
     if (k == 0) continue;
     s.push_back(src[i]); d.push_back(dst[i]); n.push_back(k);
   }
-  for (int64_t r : written) TORCH_CHECK(read.count(r) == 0, "cache_copy: row ", r, " is read and written");
+  std::sort(read.begin(), read.end());
+  std::sort(written.begin(), written.end());
+  for (size_t i = 0, j = 0; i < written.size(); ++i) {
+    TORCH_CHECK(i == 0 || written[i] != written[i - 1], "cache_copy: row ", written[i], " is written twice");
+    while (j < read.size() && read[j] < written[i]) ++j;
+    TORCH_CHECK(j == read.size() || read[j] != written[i], "cache_copy: row ", written[i], " is read and written");
+  }
   if (base.empty() || s.empty()) return;
   c10::cuda::CUDAGuard guard(first.device());
   auto stream = at::cuda::getCurrentCUDAStream();

@@ -543,36 +543,65 @@ __global__ void __launch_bounds__(sp::JOIN_WARPS * 32) shared_join_kernel(const 
   const int n = min(p.seq_lens[b], p.width), slots = has_prefix(r, n, p.slots, p.G) ? r.z : 0, row = r.w + h - kvh * p.G;
   const int own_total = own_tiles(slots > 0 ? r.x : 0, n), per = run_tiles(own_total, p.runs), owns = (own_total + per - 1) / per;
   const size_t found = (static_cast<size_t>(r.y) * p.hkv + kvh) * sp::ROWS + row, next = static_cast<size_t>(p.hkv) * sp::ROWS;
+  const int c = lane * E, mine = (slots - part + W - 1) / W, theirs = (owns - part + W - 1) / W;      // this warp's pieces and runs: part, part + W, …
+  const float *pieces = p.part + (found + part * next) * D + ((c >> 2 ^ (row & 7)) << 2 | (c & 3)), *runs = p.own_part + (part * static_cast<size_t>(p.total) + at) * D + c;
+  const size_t piece = W * next * D, run = W * static_cast<size_t>(p.total) * D;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  // its own runs: lane k holds the k-th
+  // lane k holds the figures of the k-th of its own runs, of 32 pieces at a time; the first outputs are asked for with them
   const float2 own = lane < owns ? p.own_stat[lane * static_cast<size_t>(p.total) + at] : make_float2(-INFINITY, 0.f);
-  float m = own.x;
-  for (int k = lane; k < slots; k += 32) m = fmaxf(m, p.stat[found + k * next].x);
+  float2 s = lane < mine ? p.stat[found + (part + lane * W) * next] : make_float2(-INFINITY, 0.f);
+  constexpr int FIRST = 4;
+  float v[2 * FIRST][E];
+  auto get = [](float (&to)[E], const float* from) {
+    if constexpr (E == 4) *reinterpret_cast<float4*>(to) = *reinterpret_cast<const float4*>(from);
+    else *reinterpret_cast<float2*>(to) = *reinterpret_cast<const float2*>(from);
+  };
+#pragma unroll
+  for (int k = 0; k < FIRST; ++k) {
+    if (k < mine) get(v[k], pieces + k * piece);
+    if (k < theirs) get(v[FIRST + k], runs + k * run);
+  }
+  float m = fmaxf(own.x, s.x);
+  if constexpr (W > 1) {
+    for (int k = lane; k < slots; k += 32) m = fmaxf(m, p.stat[found + k * next].x);      // the other warps' too
+  } else {
+    for (int k = lane + 32; k < slots; k += 32) m = fmaxf(m, p.stat[found + k * next].x);
+  }
   m = warp_max(m);
   float acc[E], l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  auto add = [&](const float* from, float w) {
-    float v[E];
-    if constexpr (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(from);
-    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(from);
+  auto add = [&](const float (&x)[E], float w) {
 #pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] = fmaf(v[e], w, acc[e]);
+    for (int e = 0; e < E; ++e) acc[e] = fmaf(x[e], w, acc[e]);
   };
-  const int c = lane * E, mine = (slots - part + W - 1) / W;      // this warp's pieces: part, part + W, …
-  const float* from = p.part + (found + part * next) * D + ((c >> 2 ^ (row & 7)) << 2 | (c & 3));
   for (int k0 = 0; k0 < mine; k0 += 32) {
-    const float2 s = k0 + lane < mine ? p.stat[found + (part + (k0 + lane) * W) * next] : make_float2(-INFINITY, 0.f);
+    if (k0 > 0) s = k0 + lane < mine ? p.stat[found + (part + (k0 + lane) * W) * next] : make_float2(-INFINITY, 0.f);
     const float w = s.x == -INFINITY ? 0.f : fast_exp2(s.x - m);
     l += s.y * w;
+    if (k0 == 0) {
+#pragma unroll
+      for (int k = 0; k < FIRST; ++k)
+        if (k < mine) add(v[k], __shfl_sync(0xffffffffu, w, k));
+    }
 #pragma unroll 8
-    for (int k = 0; k < min(32, mine - k0); ++k) add(from + (k0 + k) * W * next * D, __shfl_sync(0xffffffffu, w, k));
+    for (int k = k0 == 0 ? FIRST : 0; k < min(32, mine - k0); ++k) {
+      float x[E];
+      get(x, pieces + (k0 + k) * piece);
+      add(x, __shfl_sync(0xffffffffu, w, k));
+    }
   }
   const float w = own.x == -INFINITY ? 0.f : fast_exp2(own.x - m);
   if (part == 0) l += own.y * w;
   l = warp_sum(l);
-#pragma unroll 4
-  for (int k = part; k < owns; k += W) add(p.own_part + (k * static_cast<size_t>(p.total) + at) * D + c, __shfl_sync(0xffffffffu, w, k));
+#pragma unroll
+  for (int k = 0; k < FIRST; ++k)
+    if (k < theirs) add(v[FIRST + k], __shfl_sync(0xffffffffu, w, part + k * W));
+  for (int k = FIRST; k < theirs; ++k) {
+    float x[E];
+    get(x, runs + k * run);
+    add(x, __shfl_sync(0xffffffffu, w, part + k * W));
+  }
   if constexpr (W > 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) s_acc[part][c + e] = acc[e];
