@@ -80,8 +80,9 @@ def test_cache_copies_that_are_refused(src, dst, tokens):
     assert torch.equal(pools[0], before)
     with pytest.raises(ValueError):
         ops.cache_copy(pools, [0, 1], [2])
-    with pytest.raises(ValueError):
-        ops.cache_copy(pools, [0, 1], [2, 3], [1])
+    for few in ([1], []):
+        with pytest.raises(ValueError):
+            ops.cache_copy(pools, [0, 1], [2, 3], few)
 
 
 # ------------------------------------------------------------------- losses
@@ -243,6 +244,14 @@ def test_forks_own_what_they_write():
     assert copies == [] and len(whole[0]) == 3
     with pytest.raises(RuntimeError):
         c.fork(whole[0], 12, [40])
+
+
+def test_sequences_of_a_group_compare_and_print():
+    from twinkle_b200.data_format import SamplingParams
+    from twinkle_b200.sampler.engine import _Seq
+    a, b = (_Seq(0, [1, 2], SamplingParams()) for _ in range(2))
+    a.origin, b.origin = a, a
+    assert a == b and 'prompt' in repr(a)
 
 
 def test_compaction_keeps_what_is_alive():

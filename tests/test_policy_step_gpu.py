@@ -102,9 +102,13 @@ def test_shared_decode_of_pages_outside_the_pool(E):
     x, sizes, shared = batch([3], [64], 20, 16, 16, 4, 128, device='cuda')
     x[3][:, 1] = x[1].shape[0]
     x[3][1, -1] = -7
-    out = ops.paged_attention_shared(*x, ops.shared_prefix(sizes, shared, 16, 16, 4))
-    assert torch.isfinite(out).all()
+    plan = ops.shared_prefix(sizes, shared, 16, 16, 4)
+    out = ops.paged_attention_shared(*x, plan)
     assert E.read_and_clear_error() != 0
+    # a cache that has such pages, of zeros
+    k, v = (torch.cat([t, torch.zeros_like(t[:1])]) for t in x[1:3])
+    table = torch.where((x[3] < 0) | (x[3] >= x[1].shape[0]), torch.full_like(x[3], x[1].shape[0]), x[3])
+    assert torch.equal(out, ops.paged_attention_shared(x[0], k, v, table, x[4], plan))
 
 
 def test_shared_decode_far_into_a_pool(E):
@@ -411,6 +415,24 @@ def test_losses_in_a_graph(E):
         lp.copy_(x['logps'])
     graph.replay()
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_losses_have_no_second_derivative(E):
+    from twinkle_b200 import ops
+    x = _policy_inputs(4, 50, 11)
+    lp = x['logps'].clone().requires_grad_()
+    for loss in (ops.policy_loss(lp, x['labels'], x['adv'], x['old'])[0], ops.preference_loss(lp, x['labels'])[0]):
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(loss, lp, create_graph=True)
+
+
+def test_policy_losses_out_of_the_kernels_range_keep_their_methods(E):
+    from twinkle_b200.loss import GRPOLoss, SAPOLoss
+    x = _policy_inputs(4, 50, 15)
+    for loss in (SAPOLoss(tau_neg=-1.0), GRPOLoss(epsilon=-0.1)):
+        before = E.launch_count()
+        loss({'labels': x['labels']}, {'logps': x['logps']}, old_logps=x['old'], advantages=[1.0] * 4)
+        assert E.launch_count() == before
 
 
 def test_losses_keep_to_what_needs_a_gradient(E):

@@ -127,7 +127,7 @@ class GRPOLoss(Loss):
     def _on_kernel(self, labels, logps, outputs) -> bool:
         ent = outputs.get('entropies')
         return ('rules' in type(self).__dict__ and logps.is_cuda and logps.dtype == torch.float32 and logps.dim() == 2 and logps.shape == labels.shape and logps.numel() > 0
-                and self.epsilon >= 0 and self.epsilon_high >= 0 and (self.entropy_coef <= 0.0 or (ent is not None and ent.shape == logps.shape)))
+                and self.epsilon >= 0 and self.epsilon_high >= 0 and min((getattr(self, n, 1) for n in ('tau_pos', 'tau_neg', 'max_completion_length'))) > 0 and (self.entropy_coef <= 0.0 or (ent is not None and ent.shape == logps.shape)))
 
     def _kernel_loss(self, labels, logps, mask, outputs, old_logps, ref_logps, advantages, kwargs) -> torch.Tensor:
         grid = lambda v: None if v is None else align_to_mask(v, mask, logps.dtype)  # noqa: E731

@@ -911,14 +911,14 @@ def cache_copy(pools, src, dst, tokens=None) -> None:
     pools = [p for p in pools if p is not None]
     if not pools:
         return
-    src, dst, tokens = (v if isinstance(v, (list, tuple)) else [int(x) for x in v] for v in (src, dst, () if tokens is None else tokens))
-    if len(src) != len(dst) or (tokens and len(tokens) != len(src)):
+    src, dst, tokens = (v if v is None or isinstance(v, (list, tuple)) else [int(x) for x in v] for v in (src, dst, tokens))
+    if len(src) != len(dst) or (tokens is not None and len(tokens) != len(src)):
         raise ValueError('cache_copy: one destination (and number of tokens) per source')
     if not src:
         return
     if _cuda(pools[0]):
-        return ext().cache_copy(pools, src, dst, tokens)
-    ref.cache_copy(pools, src, dst, tokens)
+        return ext().cache_copy(pools, src, dst, tokens or [])
+    ref.cache_copy(pools, src, dst, tokens or ())
 
 
 def cache_write(k_pool, v_pool, rows, k, v) -> None:

@@ -39,6 +39,23 @@ struct Smem {
 };
 }  // namespace sp
 
+// mbar_wait of common.cuh, but a page outside the pool is no reason to give up: its tokens count as zeros.
+__device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, int* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  for (uint32_t it = 0;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 0x3ff) == 0x3ff) {
+      if (global_timer_ns() - t0 > 2000000000ull) {
+        atomicCAS(err, 0, ERR_ATTN_WAIT);
+        return false;
+      }
+      const int e = *reinterpret_cast<volatile int*>(err);
+      if (e != 0 && e != ERR_BOUNDS) return false;       // someone else already gave up
+    }
+  }
+}
+
 struct SharedPrefix {
   const int* items;        // [items][8]: first sequence, sequences, first block of 128 tokens, blocks, tokens of the prefix, slot
   const int* tables;
@@ -136,7 +153,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         places = ahead;
         ahead = lookup(j * boxes + 32 + lane);
       }
-      if (j >= NS && !__all_sync(0xffffffffu, mbar_wait(&empty[st], (j / NS - 1) & 1, p.err, ERR_ATTN_WAIT))) break;
+      if (j >= NS && !__all_sync(0xffffffffu, shared_wait(&empty[st], (j / NS - 1) & 1, p.err))) break;
       if (elect_one()) mbar_expect_tx(&full[st], S::TILE);
       __syncwarp();
       for (int u = 0; u < boxes; ++u) {
@@ -154,7 +171,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     constexpr uint32_t idesc_s = umma_idesc_bf16(ROWS, BKV, false, false);
     constexpr uint32_t idesc_o = umma_idesc_bf16(ROWS, D, false, true);
     const uint64_t dq = umma_desc(smem_u32(smem + S::Q), 16, 1024);
-    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, p.err, ERR_ATTN_WAIT)); };
+    auto wait = [&](uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, shared_wait(bar, parity, p.err)); };
     auto scores = [&](int j) -> bool {
       const int st = j % NS, t = j & 1;
       if (!wait(&k_full[st], (j / NS) & 1)) return false;
@@ -201,7 +218,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     float2 l2 = make_float2(0.f, 0.f);
     bool dead = false;
     for (int j = t; j < n; j += 2) {
-      if (!mbar_wait(&s_full[t], (j >> 1) & 1, p.err, ERR_ATTN_WAIT)) { dead = true; break; }
+      if (!shared_wait(&s_full[t], (j >> 1) & 1, p.err)) { dead = true; break; }
       if (idle) {
         mbar_arrive(&p_ready[t]);
         continue;
@@ -282,7 +299,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     float* xo = reinterpret_cast<float*>(smem + S::K);
     float* xs = reinterpret_cast<float*>(smem + S::Q);
     const bool two = n > 1;
-    dead = dead || !mbar_wait(&o_done[0], 0, p.err, ERR_ATTN_WAIT) || (two && !mbar_wait(&o_done[1], 0, p.err, ERR_ATTN_WAIT));
+    dead = dead || !shared_wait(&o_done[0], 0, p.err) || (two && !shared_wait(&o_done[1], 0, p.err));
     tc_fence_after();
     const float l = l2.x + l2.y;
     auto place = [&](int c) { return reinterpret_cast<float4*>(xo + row * D + ((c ^ (row & 7)) << 2)); };
@@ -677,7 +694,7 @@ torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc,
               "caches [blocks,bs,Hkv,D] bf16 of one shape");
   const int64_t B = q.size(0), hq = q.size(1), D = q.size(2), hkv = kc.size(2), bs = kc.size(1), G = hkv > 0 ? hq / hkv : 0;
   TORCH_CHECK(kc.size(3) == D && (D == 64 || D == 128) && hkv > 0 && hq % hkv == 0 && G >= 1 && G <= sp::ROWS && bs % 8 == 0 && bs > 0, "heads of 64 or 128, pages of a multiple of 8 tokens");
-  TORCH_CHECK(kc.size(0) * bs < (int64_t(1) << 31) - sp::ROWS && hkv <= 65535 && B <= 65535, "pools of up to 2^31 rows");
+  TORCH_CHECK(kc.size(0) * bs < (int64_t(1) << 31) - sp::ROWS && hkv * ((G + ow::HEADS - 1) / ow::HEADS) <= 65535 && B <= 65535, "pools of up to 2^31 rows, 65535 sequences");
   for (const auto* t : {&q, &kc, &vc}) TORCH_CHECK(t->device() == q.device() && reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "q and caches on one device and on 16-byte boundaries");
   for (const auto* t : {&tables, &seq_lens, &plan}) TORCH_CHECK(t->device() == q.device() && t->scalar_type() == torch::kInt32 && t->is_contiguous(), "int32 tables, lengths and plan on the device of q");
   TORCH_CHECK(tables.dim() == 2 && tables.size(0) == B && seq_lens.numel() == B, "a row of the table and a length per sequence");

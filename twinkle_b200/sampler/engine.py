@@ -167,7 +167,7 @@ class _Seq:
     vision: Optional[Dict[str, Any]] = None   # pixel_values, image_grid_thw, mrope_position_ids [3, L] of a prompt with images
     rope_delta: int = 0                        # rotary position − token index for the tokens after the prompt (images compress positions)
     linear: Dict[int, Tuple[torch.Tensor, torch.Tensor]] = field(default_factory=dict)  # layer → (conv rows, recurrent state) of linear-attention layers
-    origin: Optional['_Seq'] = None            # the sequence whose prompt this one shares (itself: others share its own)
+    origin: Optional['_Seq'] = field(default=None, compare=False, repr=False)    # the sequence whose prompt this one shares (itself: others share its own)
 
     @property
     def length(self) -> int:
