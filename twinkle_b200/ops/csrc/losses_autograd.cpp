@@ -1,4 +1,5 @@
-// Autograd of the losses in losses.cu.  A micro-batch's kernels take 10 us; through a Function in Python a step spent 115 us on the host, here 60.
+// Autograd of the losses in losses.cu.  A micro-batch's kernels take 12 us, so a step's time is the host's: 115 us through a Function in Python, 80 to 90 here, 50 of which torch's
+// engine takes for any gradient.
 #include <torch/extension.h>
 
 namespace tk {
