@@ -1108,7 +1108,7 @@ def fused_linear_logprob(hidden, weight, labels, temperature: float = 1.0, with_
 
 
 # ------------------------------------------------------------------ losses
-_POLICY = {'ratio': ('token', 'sequence'), 'surrogate': ('clip', 'soft', 'weight'), 'reduce': ('sequence', 'token', 'sum')}
+_RATIO, _SURROGATE, _REDUCE = {'token': 0, 'sequence': 1}, {'clip': 0, 'soft': 1, 'weight': 2}, {'sequence': 0, 'token': 1, 'sum': 2}
 _PREFERENCE = ('sigmoid', 'hinge', 'ipo', 'kto_pair', 'simpo', 'orpo')
 
 
@@ -1142,9 +1142,10 @@ def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entro
     for ``ratio='sequence'``, and ``r = e^l`` a token costs ``−min(r A, clamp(r, 1 − epsilon, 1 + epsilon_high) A)`` (``clip``), ``−σ(τ (r − 1)) 4 A / τ`` with ``τ`` by the sign of A (``soft``) or
     ``−min(r, 1 + epsilon) A logp`` with the weight held fixed (``weight``), plus ``beta (e^d − d − 1)`` with ``d = ref − logp``, minus ``entropy_coef`` times its entropy.  ``reduce``: mean over rows of
     each row's mean, sum over the number of tokens, or sum over ``denominator``.  ``stats``: KL to the old policy, shares of tokens below and above the bounds, number of tokens."""
-    for name, value in (('ratio', ratio), ('surrogate', surrogate), ('reduce', reduce)):
-        if value not in _POLICY[name]:
-            raise ValueError(f'policy_loss: {name} is one of {_POLICY[name]}, not {value!r}')
+    try:
+        rules = _RATIO[ratio], _SURROGATE[surrogate], _REDUCE[reduce]
+    except KeyError as e:
+        raise ValueError(f'policy_loss: no {e.args[0]!r} among the ratios {list(_RATIO)}, surrogates {list(_SURROGATE)} and reductions {list(_REDUCE)}') from None
     epsilon_high = epsilon if epsilon_high is None else epsilon_high
     if not 0 <= epsilon or not 0 <= epsilon_high or not denominator > 0 or not all(t > 0 for t in tau):
         raise ValueError('policy_loss: bounds of zero or more, a positive denominator and positive temperatures')
@@ -1156,7 +1157,7 @@ def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entro
     constants = [t for t in (advantages, old_logps, ref_logps) if t is not None]
     if _cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not (torch.is_grad_enabled() and any(t.requires_grad for t in constants)):
         loss, stats = ext().policy_loss(_side_by_side(logps), _side_by_side(entropies), _side_by_side(labels), _side_by_side(advantages), _side_by_side(old_logps), _side_by_side(ref_logps),
-                                        _POLICY['ratio'].index(ratio), _POLICY['surrogate'].index(surrogate), _POLICY['reduce'].index(reduce), epsilon, epsilon_high, beta, entropy_coef, *tau,
+                                        *rules, epsilon, epsilon_high, beta, entropy_coef, *tau,
                                         denominator, ignore_index)
         return loss, stats
     return ref.policy_loss(logps, labels, advantages, old_logps, ref_logps, entropies, ratio, surrogate, reduce, epsilon, epsilon_high, beta, entropy_coef, tau, denominator, ignore_index)

@@ -225,7 +225,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     float2 l2 = make_float2(0.f, 0.f);
     bool dead = false;
     for (int j = t; j < n; j += 2) {
-      if (!shared_wait(&s_full[t], (j >> 1) & 1, p.err)) { dead = true; break; }
+      if (!__all_sync(0xffffffffu, shared_wait(&s_full[t], (j >> 1) & 1, p.err))) { dead = true; break; }      // a warp stays together
       if (idle) {
         mbar_arrive(&p_ready[t]);
         continue;
@@ -306,7 +306,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     float* xo = reinterpret_cast<float*>(smem + S::K);
     float* xs = reinterpret_cast<float*>(smem + S::Q);
     const bool two = n > 1;
-    dead = dead || !shared_wait(&o_done[0], 0, p.err) || (two && !shared_wait(&o_done[1], 0, p.err));
+    dead = dead || !__all_sync(0xffffffffu, shared_wait(&o_done[0], 0, p.err)) || (two && !__all_sync(0xffffffffu, shared_wait(&o_done[1], 0, p.err)));
     tc_fence_after();
     const float l = l2.x + l2.y;
     auto place = [&](int c) { return reinterpret_cast<float4*>(xo + row * D + ((c ^ (row & 7)) << 2)); };
@@ -400,9 +400,9 @@ __global__ void __launch_bounds__(ow::WARPS * 32, 3) own_pages_kernel(const OwnP
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // one CTA sees the prefix kernel end, so that this kernel ends after it
   auto leave = [] {
-    if (blockIdx.x == 0 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (blockIdx.x == gridDim.x - 1 && blockIdx.y == gridDim.y - 1 && blockIdx.z == gridDim.z - 1) asm volatile("griddepcontrol.wait;" ::: "memory");
   };
-  const int groups = (p.G + HEADS - 1) / HEADS, kvh = blockIdx.y / groups, g0 = blockIdx.y % groups * HEADS, h0 = kvh * p.G + g0, GH = min(HEADS, p.G - g0), b = blockIdx.z, run = blockIdx.x;
+  const int groups = (p.G + HEADS - 1) / HEADS, kvh = blockIdx.x / groups, g0 = blockIdx.x % groups * HEADS, h0 = kvh * p.G + g0, GH = min(HEADS, p.G - g0), b = blockIdx.y, run = blockIdx.z;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, quad = lane & 3, hrow = lane >> 2;
   const int4 line = reinterpret_cast<const int4*>(p.rows)[b];
   const int n = min(p.seq_lens[b], p.max_blocks * p.block_size), first = has_prefix(line, n, p.slots, p.G) ? line.x : 0;
@@ -688,7 +688,7 @@ static void launch_own(const OwnPages& p, cudaStream_t stream) {
     TK_CUDA_CHECK(cudaFuncSetAttribute(own_pages_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ow::smem_bytes<D>()));
     TK_CUDA_CHECK(cudaFuncSetAttribute(own_pages_kernel<D>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
   });
-  launch_beside(own_pages_kernel<D>, dim3(p.runs, p.hkv * ((p.G + ow::HEADS - 1) / ow::HEADS), p.B), ow::WARPS * 32, ow::smem_bytes<D>(), p, stream);
+  launch_beside(own_pages_kernel<D>, dim3(p.hkv * ((p.G + ow::HEADS - 1) / ow::HEADS), p.B, p.runs), ow::WARPS * 32, ow::smem_bytes<D>(), p, stream);
 }
 
 template <int D, int W>
@@ -697,7 +697,8 @@ static void launch_join(const SharedJoin& p, cudaStream_t stream) {
   launch_beside(shared_join_kernel<D, W>, dim3((p.total + HEADS - 1) / HEADS), sp::JOIN_WARPS * 32, 0, p, stream);
 }
 
-// One query token per sequence; pieces: slots of a sequence at most; room: tokens that most sequences have at most beside their prefix (what their split is chosen by); plan int32 [items · 8 + B · 4]: the items, then for every sequence the tokens of its prefix, its first slot, its slots and its row in them.
+// One query token per sequence; pieces: slots of a sequence at most; room: tokens that most sequences have at most beside their prefix (what their split is chosen by); plan int32
+// [items · 8 + B · 4]: the items, then for every sequence the tokens of its prefix, its first slot, its slots and its row in them.
 torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& vc, const torch::Tensor& tables, const torch::Tensor& seq_lens, const torch::Tensor& plan,
                                 int64_t items, int64_t slots, int64_t pieces, int64_t room, double scale) {
   TORCH_CHECK(q.is_cuda() && q.scalar_type() == torch::kBFloat16 && q.is_contiguous() && q.dim() == 3, "q [B,Hq,D] bf16");
@@ -713,8 +714,14 @@ torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc,
   TORCH_CHECK(reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0 && tables.size(1) * bs < (int64_t(1) << 31), "plan on a 16-byte boundary, contexts below 2^31");
   c10::cuda::CUDAGuard guard(q.device());
   auto out = torch::empty_like(q);
-  const auto f32 = q.options().dtype(torch::kFloat32);
-  auto part = torch::empty({slots, hkv, sp::ROWS, D}, f32), stat = torch::empty({slots, hkv, sp::ROWS, 2}, f32);
+  // CTAs of a sequence's own part, by what most have (where there is more a CTA's run is longer): 256 tokens each, more where that makes over 14 CTAs per SM
+  const int64_t wide = B * hkv * ((G + ow::HEADS - 1) / ow::HEADS);
+  int64_t runs = std::max<int64_t>(1, std::min<int64_t>(ow::RUNS, (room + ow::RUN * ow::TILE - 1) / (ow::RUN * ow::TILE)));
+  while (runs > 1 && wide * runs > 14 * num_sms()) runs = (runs + 1) / 2;
+  // one workspace: outputs of the pieces and of the runs, then their figures
+  const int64_t pieces_rows = slots * hkv * sp::ROWS, runs_rows = runs * B * hq;
+  auto work = torch::empty({(pieces_rows + runs_rows) * (D + 2)}, q.options().dtype(torch::kFloat32));
+  float *part = work.data_ptr<float>(), *own_part = part + pieces_rows * D, *stat = own_part + runs_rows * D, *own_stat = stat + pieces_rows * 2;
   const int64_t box = std::min<int64_t>(bs & -bs, sp::BKV);      // the largest power of two that divides a page
   const CUtensorMap tq = make_tmap_3d(q.data_ptr(), D, hq, B, D, hq * D, 64, G, sp::ROWS / G);
   const uint64_t dims[5] = {64, 8, static_cast<uint64_t>(D / 64), static_cast<uint64_t>(hkv), static_cast<uint64_t>(kc.size(0) * bs / 8)};
@@ -722,19 +729,14 @@ torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc,
   const uint32_t boxes[5] = {64, 8, static_cast<uint32_t>(D / 64), 1, static_cast<uint32_t>(box / 8)};
   const CUtensorMap tk_ = make_tmap_5d(kc.data_ptr(), dims, strides, boxes), tv = make_tmap_5d(vc.data_ptr(), dims, strides, boxes);
   SharedPrefix p{};
-  p.items = plan.data_ptr<int>(); p.tables = tables.data_ptr<int>(); p.part = part.data_ptr<float>(); p.stat = reinterpret_cast<float2*>(stat.data_ptr<float>());
+  p.items = plan.data_ptr<int>(); p.tables = tables.data_ptr<int>(); p.part = part; p.stat = reinterpret_cast<float2*>(stat);
   p.max_blocks = tables.size(1); p.block_size = bs; p.box = box; p.num_blocks = kc.size(0); p.hkv = hkv; p.G = G; p.sequences = B; p.slots = slots;
   p.scale_log2 = static_cast<float>(scale * 1.4426950408889634); p.err = error_word();
   auto stream = at::cuda::getCurrentCUDAStream();
   if (D == 128) launch_prefix<128>(p, items, tq, tk_, tv, stream); else launch_prefix<64>(p, items, tq, tk_, tv, stream);
   const int* rows = plan.data_ptr<int>() + items * sp::ITEM;
-  // CTAs of a sequence's own part, by what most have (where there is more a CTA's run is longer): 256 tokens each, more where that makes over 14 CTAs per SM
-  const int64_t wide = B * hkv * ((G + ow::HEADS - 1) / ow::HEADS);
-  int64_t runs = std::max<int64_t>(1, std::min<int64_t>(ow::RUNS, (room + ow::RUN * ow::TILE - 1) / (ow::RUN * ow::TILE)));
-  while (runs > 1 && wide * runs > 14 * num_sms()) runs = (runs + 1) / 2;
-  auto own_part = torch::empty({runs, B, hq, D}, f32), own_stat = torch::empty({runs, B, hq, 2}, f32);
   const OwnPages own{reinterpret_cast<const bf16*>(q.data_ptr()), reinterpret_cast<const bf16*>(kc.data_ptr()), reinterpret_cast<const bf16*>(vc.data_ptr()), tables.data_ptr<int>(),
-                     seq_lens.data_ptr<int>(), rows, own_part.data_ptr<float>(), reinterpret_cast<float2*>(own_stat.data_ptr<float>()), static_cast<int>(B), static_cast<int>(hq),
+                     seq_lens.data_ptr<int>(), rows, own_part, reinterpret_cast<float2*>(own_stat), static_cast<int>(B), static_cast<int>(hq),
                      static_cast<int>(hkv), static_cast<int>(G), static_cast<int>(bs), static_cast<int>(tables.size(1)), static_cast<int>(kc.size(0)), static_cast<int>(slots), static_cast<int>(runs),
                      p.scale_log2, p.err};
   if (D == 128) launch_own<128>(own, stream); else launch_own<64>(own, stream);
