@@ -384,6 +384,33 @@ def make(op: str, a) -> Tuple[Callable[[], None], float, float]:
         seen = min(ctx, a.window or ctx) if not a.chunk else (ctx - 1) % a.chunk + 1
         return ((lambda: ops.paged_attention_decode(q, kc, vc, tables, lens, window=a.window or None, chunk=a.chunk, sinks=sinks, gate=gate, terms=terms)), 0.0,
                 2.0 * 2 * B * seen * a.kv_heads * a.width)
+    if op == 'paged_shared':
+        # --batch sequences in groups of --samples behind prompts of --seq tokens, --own tokens each (the like kernel: paged_decode)
+        B, bs, n = a.batch, 16, a.samples
+        shared, own = a.seq // bs, (a.own + bs - 1) // bs
+        groups = (B + n - 1) // n
+        kc = torch.randn(groups * shared + B * own, bs, a.kv_heads, a.width, device=dev, dtype=bf)
+        vc = torch.randn_like(kc)
+        common = torch.arange(groups * shared, dtype=torch.int32).view(groups, shared).repeat_interleave(n, 0)[:B]
+        tables = torch.cat([common, groups * shared + torch.arange(B * own, dtype=torch.int32).view(B, own)], 1).to(dev)
+        lens = torch.full((B, ), shared * bs + a.own, device=dev, dtype=torch.int32)
+        q = torch.randn(B, a.heads, a.width, device=dev, dtype=bf)
+        sizes = [min(n, B - g * n) for g in range(groups)]
+        plan = ops.shared_prefix(sizes, [shared] * groups, bs, a.heads, a.kv_heads)
+        return ((lambda: ops.paged_attention_shared(q, kc, vc, tables, lens, plan)), 4.0 * a.heads * a.width * B * (shared * bs + a.own),
+                4.0 * a.kv_heads * a.width * (groups * shared * bs + B * a.own))
+    if op == 'cache_copy':
+        # --batch pages of 16 tokens in the pools of 28 layers
+        pools = [torch.randn(2 * a.batch, 16, a.kv_heads, a.width, device=dev, dtype=bf) for _ in range(56)]
+        src, dst = list(range(a.batch)), list(range(a.batch, 2 * a.batch))
+        return (lambda: ops.cache_copy(pools, src, dst)), 0.0, 2.0 * 56 * a.batch * 16 * a.kv_heads * a.width * 2
+    if op in ('policy_loss', 'preference_loss'):
+        # --batch rows of --seq tokens, forward and backward
+        lp = -torch.rand(a.batch, a.seq, device=dev)
+        old, labels, adv = lp + 0.1 * torch.randn_like(lp), torch.ones(a.batch, a.seq, dtype=torch.int64, device=dev), torch.randn(a.batch, device=dev)
+        lp.requires_grad_()
+        loss = (lambda: ops.policy_loss(lp, labels, adv, old)[0]) if op == 'policy_loss' else (lambda: ops.preference_loss(lp, labels, old)[0])
+        return (lambda: torch.autograd.grad(loss(), lp)), 0.0, 20.0 * a.batch * a.seq
     if op == 'sample':
         lg = torch.randn(a.batch, a.vocab, device=dev)
         seeds = torch.arange(a.batch, device=dev, dtype=torch.int64)
@@ -470,6 +497,8 @@ def main() -> None:
     ap.add_argument('--hidden', type=int, default=4096)
     ap.add_argument('--vocab', type=int, default=151936)
     ap.add_argument('--batch', type=int, default=256)
+    ap.add_argument('--samples', type=int, default=8, help='paged_shared: sequences of a prompt')
+    ap.add_argument('--own', type=int, default=512, help='paged_shared: tokens of a sequence behind its prompt')
     ap.add_argument('--rank', type=int, default=16)
     ap.add_argument('--numel', type=int, default=1 << 28)
     ap.add_argument('--iters', type=int, default=10)
