@@ -417,6 +417,17 @@ def test_losses_in_a_graph(E):
     assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
+@pytest.mark.parametrize('up', [math.inf, math.nan])
+def test_masked_tokens_have_no_gradient_whatever_the_losses_is(E, up):
+    from twinkle_b200 import ops
+    x = _policy_inputs(4, 300, 16)
+    lp, en = x['logps'].clone().requires_grad_(), x['ent'].clone().requires_grad_()
+    losses = (ops.policy_loss(lp, x['labels'], x['adv'], x['old'], x['ref'], en, beta=0.1, entropy_coef=0.1)[0], ops.preference_loss(lp, x['labels'], x['ref'])[0])
+    for loss in losses:
+        for g in torch.autograd.grad(loss * up, (lp, en), allow_unused=True):
+            assert g is None or (not g[x['labels'] == -100].any() and not torch.isfinite(g[x['labels'] != -100]).any())
+
+
 def test_losses_have_no_second_derivative(E):
     from twinkle_b200 import ops
     x = _policy_inputs(4, 50, 11)

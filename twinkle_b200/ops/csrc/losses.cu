@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(ls::THREADS) policy_grad_kernel(const float* _
     for (int u = 0; u < UNROLL; ++u) {
       const int t = t0 + u * step;
       if (t >= S) break;
-      if (grad != nullptr) grad[b * S + t] = d[u] * w;
+      if (grad != nullptr) grad[b * S + t] = d[u] == 0.f ? 0.f : d[u] * w;      // masked tokens have none, whatever the gradient of the loss is
       if (grad_ent != nullptr) grad_ent[b * S + t] = label[u] != tokens.ignore ? -entropy * w : 0.f;
     }
   }
