@@ -83,7 +83,9 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   const int* item = p.items + blockIdx.x * ITEM;
   const int row0 = item[0], seqs = item[1], tile0 = item[2], n = item[3], tokens = item[4], slot = item[5], kvh = blockIdx.y;
   if (n <= 0) return;                      // an item that fills up a captured plan
-  if (row0 < 0 || row0 >= p.sequences || tile0 < 0 || slot < 0 || slot >= p.slots || tokens > p.max_blocks * p.block_size) {      // not a plan for these sequences
+  // not a plan for these sequences: rows beyond a slot, sequences, blocks or tokens that are not there (differences only: no sum of a plan's numbers wraps)
+  if (seqs < 1 || seqs > ROWS / p.G || row0 < 0 || row0 > p.sequences - seqs || slot < 0 || slot >= p.slots || tokens < 1 || tokens > p.max_blocks * p.block_size || tile0 < 0 ||
+      n > (tokens - 1) / BKV + 1 - tile0) {
     if (threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BOUNDS);
     return;
   }
@@ -366,7 +368,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
 // A sequence has a part in its group's prefix when it is as long (`r`: its line of the plan); else it attends to all of its own keys.
 __device__ __forceinline__ bool has_prefix(const int4& r, int n, int slots, int group) {
-  return n >= r.x && r.x >= 0 && r.z > 0 && r.y >= 0 && r.y + r.z <= slots && r.w >= 0 && r.w + group <= sp::ROWS;
+  return n >= r.x && r.x >= 0 && r.z > 0 && r.y >= 0 && r.z <= slots - r.y && r.w >= 0 && r.w <= sp::ROWS - group;
 }
 // The sequences' own pages: a CTA per run of 16 tiles of 16 tokens or more of a sequence, key head and eight query heads; tiles go round robin over its four warps, each with rings of
 // two tiles of keys and two of values filled by cp.async.  Products as in paged_decode.cu: heads are rows 0–7, rows 8–15 take what rounding the probabilities left.  Its CTAs fit an SM
