@@ -830,7 +830,7 @@ class SharedPrefix(NamedTuple):
 
 
 def _prefix_items(sizes, blocks, block_size: int, group: int, kv_heads: int, sms: int):
-    """Pieces of work ``[first sequence, sequences, first block of 128 tokens, blocks of 128, tokens, slot]`` and per sequence ``[tokens, first slot, slots, row]``.
+    """Pieces of work ``[first sequence, sequences, first block of 128 tokens, blocks of 128, tokens, slot, first sequence of the group]`` and per sequence ``[tokens, first slot, slots, row]``.
 
     A tile of query rows holds ``128 // group`` sequences of one group.  Every SM runs one piece of one key head at a time; a piece costs its blocks and about two blocks'
     time to begin and end.  Of all lengths of a piece the one is taken whose waves over the SMs cost least."""
@@ -840,7 +840,7 @@ def _prefix_items(sizes, blocks, block_size: int, group: int, kv_heads: int, sms
         tokens, parts = b * block_size, (n + per - 1) // per
         for i in range(parts if tokens else 0):      # a group's tiles are even
             lo, hi = n * i // parts, n * (i + 1) // parts
-            tiles.append((at + lo, hi - lo, tokens, (tokens + 127) // 128))
+            tiles.append((at + lo, hi - lo, tokens, (tokens + 127) // 128, at))
         at += n
     if not tiles:
         return [], lines
@@ -854,13 +854,13 @@ def _prefix_items(sizes, blocks, block_size: int, group: int, kv_heads: int, sms
         if best is None or cost < best[0]:
             best = (cost, cut)
     items, slot = [], 0
-    for row, n, tokens, length in tiles:
+    for row, n, tokens, length, first in tiles:
         parts = (length + best[1] - 1) // best[1]
         for i in range(n):
             lines[row + i] = [tokens, slot, parts, i * group]
         for i in range(parts):
             lo, hi = length * i // parts, length * (i + 1) // parts
-            items.append([row, n, lo, hi - lo, tokens, slot, 0, 0])
+            items.append([row, n, lo, hi - lo, tokens, slot, first, 0])
             slot += 1
     return items, lines
 
@@ -887,8 +887,8 @@ def prefix_items(sequences: int, kv_heads: int, device='cuda') -> int:
 
 
 def paged_attention_shared(q, k_cache, v_cache, block_tables, seq_lens, prefix: SharedPrefix, scale: Optional[float] = None):
-    """``paged_attention_decode`` for sequences that share pages: the shared ones are read once per group.  The table rows of a group begin with the same pages and
-    the first sequence of a group is a live one; a sequence shorter than what its group shares attends to its own length.  A page outside the pools counts as zeros and sets the error word.
+    """``paged_attention_decode`` for sequences that share pages: the shared ones are read once per group.  The shared ones are those that the
+    table row of a group's first sequence names, whose length may be anything; a sequence that is shorter than what its group shares (0: a finished one) attends to its own length of its own row.  A page outside the pools counts as zeros and sets the error word.
 
     bf16 caches of one width, 64 or 128, with pages of a multiple of 8 tokens; the rest goes through ``paged_attention_decode``, which reads all pages per sequence."""
     if prefix.sequences != q.shape[0] or prefix.heads != q.shape[1] or prefix.kv_heads != k_cache.shape[2] or prefix.block_size != k_cache.shape[1]:

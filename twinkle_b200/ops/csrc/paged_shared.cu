@@ -64,7 +64,7 @@ __device__ __forceinline__ bool shared_wait(uint64_t* bar, uint32_t parity, int*
 }
 
 struct SharedPrefix {
-  const int* items;        // [items][8]: first sequence, sequences, first block of 128 tokens, blocks, tokens of the prefix, slot
+  const int* items;        // [items][8]: first sequence, sequences, first block of 128 tokens, blocks, tokens of the prefix, slot, first sequence of the group (whose row names the pages)
   const int* tables;
   float* part;             // [slots, hkv, 128, D], four columns c of row r at c ^ (r & 7)
   float2* stat;            // [slots, hkv, 128] maximum (log2 units), sum
@@ -81,11 +81,11 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   constexpr int NS = S::STAGES, CH = D / 64;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int* item = p.items + blockIdx.x * ITEM;
-  const int row0 = item[0], seqs = item[1], tile0 = item[2], n = item[3], tokens = item[4], slot = item[5], kvh = blockIdx.y;
+  const int row0 = item[0], seqs = item[1], tile0 = item[2], n = item[3], tokens = item[4], slot = item[5], named = item[6], kvh = blockIdx.y;
   if (n <= 0) return;                      // an item that fills up a captured plan
   // not a plan for these sequences: rows beyond a slot, sequences, blocks or tokens that are not there (differences only: no sum of a plan's numbers wraps)
   if (seqs < 1 || seqs > ROWS / p.G || row0 < 0 || row0 > p.sequences - seqs || slot < 0 || slot >= p.slots || tokens < 1 || tokens > p.max_blocks * p.block_size || tile0 < 0 ||
-      n > (tokens - 1) / BKV + 1 - tile0) {
+      n > (tokens - 1) / BKV + 1 - tile0 || named < 0 || named > row0) {
     if (threadIdx.x == 0) atomicCAS(p.err, 0, ERR_BOUNDS);
     return;
   }
@@ -139,7 +139,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     auto lookup = [&](int box) -> int {
       const int t = tile0 * BKV + box * p.box;
       if (box >= n * boxes || t >= tokens) return outside;
-      const int block = p.tables[static_cast<size_t>(row0) * p.max_blocks + t / p.block_size];
+      const int block = p.tables[static_cast<size_t>(named) * p.max_blocks + t / p.block_size];
       if (block < 0 || block >= p.num_blocks) {      // whoever reads the word next raises
         atomicCAS(p.err, 0, ERR_BOUNDS);
         return outside;
