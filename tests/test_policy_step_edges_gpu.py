@@ -52,3 +52,40 @@ def test_finished_sequences_stay_in_their_group(E):  # noqa: F811
     out = ops.paged_attention_shared(*x, plan)
     close(out, *attention(*x))
     assert not out[done + [0]].any()
+
+
+# --------------------------------------------------------------------- losses
+def test_kl_term_of_any_size(E):  # noqa: F811
+    """One token alone, ratio one and no advantage.  Its loss is e^d − d − 1: up to |d| = 1 a series with a rounded sum and two products (3.5 roundings of 2^-24), beyond that e^d − 1 with an
+    error of at most 2^-23 of itself, less d: 5.4 · 2^-24 at e^d − 1 = 2.  Its derivative 1 − e^d has the series' error times rest / (e^d − 1) < 0.6 and a rounding, or 2^-23."""
+    from twinkle_b200 import ops
+    d = torch.cat([torch.linspace(-2, 2, 401), *(c + torch.linspace(-0.02, 0.02, 41) for c in (-1, -0.5, 0.5, 1)), torch.tensor([-15.0, -4.0, 4.0, 15.0])]).cuda()
+    zero, one = torch.zeros(1, device='cuda'), torch.ones(1, len(d), dtype=torch.bool, device='cuda')
+    wide = d.double()
+    rest = torch.expm1(wide) - wide
+    rest = torch.where(wide.abs() < 0.1, sum(wide**k / math.factorial(k) for k in range(2, 12)), rest)
+    got = torch.stack([ops.policy_loss(zero[None], one[:, :1], zero, None, x.view(1, 1), beta=1.0)[0] for x in d]).double()
+    assert ((got - rest).abs() <= 2**-21.5 * rest).all()
+    lp = torch.zeros(1, len(d), device='cuda', requires_grad=True)
+    g = torch.autograd.grad(ops.policy_loss(lp, one, zero, None, d[None], beta=1.0, reduce='sum')[0], lp)[0][0].double()
+    assert ((g + torch.expm1(wide)).abs() <= 2**-22 * torch.expm1(wide).abs()).all()
+
+
+def test_kl_gradient_of_tokens_that_the_reference_rules_out(E):  # noqa: F811
+    """d = −∞ and far below: e^d − 1 is −1."""
+    from twinkle_b200 import ops
+    lp = torch.full((1, 4), -1.0, device='cuda', requires_grad=True)
+    ref = torch.tensor([[-math.inf, -1e9, -200.0, -1.0]], device='cuda')
+    loss = ops.policy_loss(lp, torch.ones(1, 4, dtype=torch.bool, device='cuda'), torch.zeros(1, device='cuda'), None, ref, beta=0.5, reduce='sum')[0]
+    assert torch.autograd.grad(loss, lp)[0].tolist() == [[0.5, 0.5, 0.5, 0.0]] and float(loss.detach()) == math.inf
+
+
+def test_ratios_are_those_of_the_exponential(E):  # noqa: F811
+    """An exponential is off by at most 2^-23 of itself; the token's other factors are one."""
+    from twinkle_b200 import ops
+    l = torch.linspace(-19, 19, 5000, device='cuda')[None]
+    for ratio, x, old in (('token', l, torch.zeros_like(l)), ):
+        lp = x.clone().requires_grad_()
+        loss, _ = ops.policy_loss(lp, torch.ones_like(l, dtype=torch.bool), torch.ones(1, device='cuda'), old, ratio=ratio, epsilon=1.0, epsilon_high=1e9, reduce='sum')
+        g = torch.autograd.grad(loss, lp)[0].double()
+        assert ((g + x.double().exp()).abs() <= 2**-22.9 * x.double().exp()).all()

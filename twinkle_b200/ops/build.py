@@ -36,6 +36,13 @@ NVCC_FLAGS = ['-gencode', 'arch=compute_100a,code=sm_100a', '-lineinfo', '-O3', 
               '-Xcompiler', '-fPIC', '--expt-relaxed-constexpr', '--expt-extended-lambda', '-DNDEBUG',
               '-U__CUDA_NO_HALF_OPERATORS__', '-U__CUDA_NO_BFLOAT16_CONVERSIONS__', '-U__CUDA_NO_HALF_CONVERSIONS__']
 
+# sources whose results are figures rather than activations: full-precision exponentials and quotients, small numbers kept
+_PRECISE = ('losses.cu', )
+
+
+def _flags(src: str) -> List[str]:
+    return [f for f in NVCC_FLAGS if f != '--use_fast_math' or os.path.basename(src) not in _PRECISE]
+
 
 def prefer_serving(parts: Sequence[str] = tuple(_PARTS)) -> None:
     """Let the serving subset with these mechanisms stand in for the full extension when that is not built (call before the first
@@ -76,7 +83,7 @@ def _digest() -> str:
     for f in _sources() + sorted(glob.glob(os.path.join(_CSRC, '*.cuh')) + glob.glob(os.path.join(_CSRC, '*.h'))):
         with open(f, 'rb') as fh:
             h.update(fh.read())
-    h.update(' '.join(NVCC_FLAGS).encode())
+    h.update(' '.join(NVCC_FLAGS + ['precise:', *_PRECISE]).encode())
     return h.hexdigest()
 
 
@@ -129,10 +136,10 @@ def _build_locked(verbose: bool, jobs: Optional[int], serving: Optional[Tuple[st
         h = hashlib.sha1(open(src, 'rb').read())
         for hdr in _local_includes(src):  # only the headers this source pulls in: touching one header rebuilds its users
             h.update(open(hdr, 'rb').read())
-        h.update(' '.join(NVCC_FLAGS + own).encode())
+        h.update(' '.join(_flags(src) + own).encode())
         if os.path.isfile(obj) and os.path.isfile(dep_stamp) and open(dep_stamp).read() == h.hexdigest():
             return obj
-        cmd = [nvcc, '-c', src, '-o', obj] + NVCC_FLAGS + inc + defs + own
+        cmd = [nvcc, '-c', src, '-o', obj] + _flags(src) + inc + defs + own
         if verbose:
             cmd += ['-Xptxas', '-v']
             print(' '.join(cmd), file=sys.stderr)

@@ -10,7 +10,8 @@
 // thread of a cluster reading the others' sums those reads took longer than the tokens (95 and 40).  On the host a step with its gradient takes 80 us, 50 of them torch's engine.
 //
 // Precision: per token in fp32, sums over tokens and rows in fp64 (a loss is a small difference of sums of advantages).  Differences of log-probs are formed in fp64 and compared
-// with the logarithms of the bounds, so that a token at a bound falls on the right side; e^d − 1 and e^d − d − 1 of small d come from their series.
+// with the logarithms of the bounds, so that a token at a bound falls on the right side; e^d − 1 and e^d − d − 1 of small d come from a series.  Exponentials and quotients are the exact
+// functions', not the fast ones': nothing here is bound by arithmetic.  The file is compiled without fast math.
 // Masked tokens are not read into any sum: infinities and NaN there have no effect.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -29,16 +30,16 @@ namespace ls {
 constexpr int THREADS = 256, UNROLL = 4, HOLD = 32, CTAS = 4;      // tokens of a batch, tokens whose terms a thread keeps, CTAs of an SM
 }
 
-// e^x to 2^-21: the rounding of x / ln 2 is carried along.
-__device__ __forceinline__ float exp_of(float x) {
-  const float t = x * 1.4426950408889634f;
-  const float rest = fmaf(x, 1.4426950408889634f, -t) + x * 1.925963033500e-8f;      // log2(e) − float(log2(e))
-  const float y = fast_exp2(t);
-  return fabsf(t) < 126.f ? fmaf(y, rest * 0.6931471805599453f, y) : y;
-}
-// e^x − x − 1: its series up to x^11 where |x| ≤ 1/2 (the next term is below 2^-26 of the sum)
-__device__ __forceinline__ float exp_rest(float x) {
-  if (fabsf(x) > 0.5f) return exp_of(x) - x - 1.f;
+// e^x − 1 and, without cancellation, e^x − 1 − x.  Where |x| ≤ 1 the latter is its series up to x^11 (the next term is below 2^-27 of the sum), three and a half roundings; beyond, the
+// difference costs at most a rounding of e^x − 1 over a third of it: both are within 2^-21.5, and the former stays finite where x is −∞.
+struct Exp {
+  float less_one, rest;
+};
+__device__ __forceinline__ Exp exp_parts(float x) {
+  if (!(fabsf(x) <= 1.f)) {
+    const float e = expm1f(x);
+    return {e, e - x};
+  }
   float r = 1.f / 39916800.f;
   r = fmaf(r, x, 1.f / 3628800.f);
   r = fmaf(r, x, 1.f / 362880.f);
@@ -49,7 +50,8 @@ __device__ __forceinline__ float exp_rest(float x) {
   r = fmaf(r, x, 1.f / 24.f);
   r = fmaf(r, x, 1.f / 6.f);
   r = fmaf(r, x, 0.5f);
-  return r * x * x;
+  r *= x * x;
+  return {r + x, r};
 }
 
 // Which tokens count: labels other than `ignore`, or a mask of bytes (ignore: 0).
@@ -136,14 +138,16 @@ struct Policy {
 };
 
 struct Ratio {
-  float r, r1, lr;        // ratio, ratio − 1, its logarithm
+  float r, r1, rest;      // ratio, ratio − 1, ratio − 1 − its logarithm
   bool below, above, over;
 };
 __device__ __forceinline__ Ratio ratio_of(const Policy& p, double l) {
   Ratio x;
-  x.lr = static_cast<float>(l);
-  x.r = exp_of(x.lr);
-  x.r1 = fabsf(x.lr) > 0.5f ? x.r - 1.f : exp_rest(x.lr) + x.lr;
+  const float lr = static_cast<float>(l);
+  const Exp e = exp_parts(lr);
+  x.r = expf(lr);
+  x.r1 = e.less_one;
+  x.rest = e.rest;
   x.below = l < p.log_lo;
   x.above = l > p.log_hi;
   x.over = l > p.log_top;
@@ -160,7 +164,7 @@ __device__ __forceinline__ void surrogate(const Policy& p, const Ratio& x, float
     by_ratio = bound ? 0.f : -x.r * a;
   } else if constexpr (KIND == SOFT) {
     const float tau = a > 0.f ? p.tau_pos : p.tau_neg;
-    const float gate = 1.f / (1.f + exp_of(-tau * x.r1));
+    const float gate = 1.f / (1.f + expf(-tau * x.r1));
     f = -gate * 4.f / tau * a;
     by_ratio = -4.f * gate * (1.f - gate) * x.r * a;
   } else {
@@ -200,9 +204,9 @@ struct Batch {
   __device__ __forceinline__ void others(const Policy& p, int u, float& f, float& by_logp) const {
     if (p.ref.p != nullptr) {
       const float d = static_cast<float>(static_cast<double>(ref[u]) - static_cast<double>(logp[u]));
-      const float e2 = exp_rest(d);
-      f += p.beta * e2;
-      by_logp -= p.beta * (e2 + d);
+      const Exp e = exp_parts(d);
+      f += p.beta * e.rest;
+      by_logp -= p.beta * e.less_one;
     }
     if (p.ent.p != nullptr) f -= p.entropy * ent[u];
   }
@@ -242,7 +246,7 @@ __global__ void __launch_bounds__(ls::THREADS, ls::CTAS) policy_token_kernel(con
         x.others(p, u, f, by_logp);
         g = (inside ? by_ratio : 0.f) + by_logp;
         f4 += f;
-        kl4 += exp_rest(r.lr);
+        kl4 += r.rest;
         ++n;
         below += r.below;
         above += r.above;
@@ -326,7 +330,7 @@ __global__ void __launch_bounds__(ls::THREADS, ls::CTAS) policy_sequence_kernel(
       }
     }
   }
-  const double out[5] = {loss, s[1], s[1] * static_cast<double>(exp_rest(r.lr)), r.below ? s[1] : 0.0, r.above ? s[1] : 0.0};
+  const double out[5] = {loss, s[1], s[1] * static_cast<double>(r.rest), r.below ? s[1] : 0.0, r.above ? s[1] : 0.0};
   put_sums(p, b, out);
 }
 
