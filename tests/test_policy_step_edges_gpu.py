@@ -89,3 +89,18 @@ def test_ratios_are_those_of_the_exponential(E):  # noqa: F811
         loss, _ = ops.policy_loss(lp, torch.ones_like(l, dtype=torch.bool), torch.ones(1, device='cuda'), old, ratio=ratio, epsilon=1.0, epsilon_high=1e9, reduce='sum')
         g = torch.autograd.grad(loss, lp)[0].double()
         assert ((g + x.double().exp()).abs() <= 2**-22.9 * x.double().exp()).all()
+
+
+def test_soft_gate_far_from_one(E):  # noqa: F811
+    """The gate times what it leaves of one: e^-|z| (1 + e^-|z|)^-2 with z = τ (r − 1), |z| up to 40.  r − 1 is within 3 · 2^-24 (1.5 · 2^-23 of itself), so z, a product, within 4 · 2^-24 |z|; e^-|z| is
+    off by that and 2^-23, the two quotients, the sum (met twice) and the products by a rounding each, the ratio by 2^-23: 4 |z| + 12 roundings of 2^-24."""
+    from twinkle_b200 import ops
+    r = torch.cat([torch.linspace(0.01, 0.99, 200), torch.linspace(1.01, 41, 800)]).double()
+    lp = r.log().float().cuda()[None].requires_grad_()
+    old, one = torch.zeros_like(lp), torch.ones_like(lp, dtype=torch.bool)
+    g = torch.autograd.grad(ops.policy_loss(lp, one, torch.ones(1, device='cuda'), old, surrogate='soft', reduce='sum')[0], lp)[0].double()
+    x = lp.detach().double()
+    z = torch.expm1(x)
+    e = torch.exp(-z.abs())
+    want = -4 * e / (1 + e)**2 * x.exp()
+    assert ((g - want).abs() <= (4 * z.abs() + 12) * 2**-24 * want.abs()).all()

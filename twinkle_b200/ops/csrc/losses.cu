@@ -164,9 +164,9 @@ __device__ __forceinline__ void surrogate(const Policy& p, const Ratio& x, float
     by_ratio = bound ? 0.f : -x.r * a;
   } else if constexpr (KIND == SOFT) {
     const float tau = a > 0.f ? p.tau_pos : p.tau_neg;
-    const float gate = 1.f / (1.f + expf(-tau * x.r1));
-    f = -gate * 4.f / tau * a;
-    by_ratio = -4.f * gate * (1.f - gate) * x.r * a;
+    const float z = tau * x.r1, e = expf(-fabsf(z)), high = 1.f / (1.f + e), low = e * high;      // the gate and what it leaves of one, neither by a difference
+    f = -(z >= 0.f ? high : low) * 4.f / tau * a;
+    by_ratio = -4.f * high * low * x.r * a;
   } else {
     const float w = (x.over ? p.top : x.r) * a;
     f = -w * logp;
