@@ -5,7 +5,7 @@ import pytest
 import torch
 
 from tests.policy_step_oracle import attention, batch
-from tests.test_policy_step_gpu import E, close  # noqa: F401   (the fixture)
+from tests.test_policy_step_gpu import E, _policy_inputs, close  # noqa: F401   (the fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -104,3 +104,41 @@ def test_soft_gate_far_from_one(E):  # noqa: F811
     e = torch.exp(-z.abs())
     want = -4 * e / (1 + e)**2 * x.exp()
     assert ((g - want).abs() <= (4 * z.abs() + 12) * 2**-24 * want.abs()).all()
+
+
+# -------------------------------------------------------------- loss classes
+@pytest.mark.parametrize('where', ['object', 'class', 'base'])
+def test_replaced_rules_are_followed(E, where, monkeypatch):  # noqa: F811
+    from twinkle_b200 import loss as L
+    x = _policy_inputs(4, 50, 15)
+    obj = L.SAPOLoss() if where == 'base' else L.GRPOLoss()
+    call = lambda: obj({'labels': x['labels']}, {'logps': x['logps']}, old_logps=x['logps'], advantages=[1.0] * 4)['loss']  # noqa: E731
+    before = E.launch_count()
+    call()
+    assert E.launch_count() > before
+    if where == 'object':
+        monkeypatch.setattr(obj, '_surrogate', lambda ratio, adv, logps: -3.0 * ratio * adv)
+    elif where == 'class':
+        monkeypatch.setattr(L.GRPOLoss, '_surrogate', lambda self, ratio, adv, logps: -3.0 * ratio * adv)
+    else:
+        monkeypatch.setattr(L.GRPOLoss, '_aggregate', lambda self, per_token, mask, **k: 3.0 * (per_token * mask).sum() / mask.sum())
+    before = E.launch_count()
+    got = float(call())
+    # a token costs −r A = −1 (SAPO: −σ(0) · 4 = −2) times three; a row without tokens nothing
+    rows = float(((x['labels'] != -100).any(-1)).float().mean())
+    assert E.launch_count() == before and got == pytest.approx(-6.0 if where == 'base' else -3.0 * rows, abs=1e-5)
+
+
+@pytest.mark.parametrize('name', ['_seq_logps', '_align_ref', '_nll'])
+def test_replaced_parts_of_a_preference_loss_are_followed(E, name, monkeypatch):  # noqa: F811
+    from twinkle_b200 import loss as L
+    x = _policy_inputs(4, 50, 15)
+    inputs, outputs, extra = {'labels': x['labels']}, {'logps': x['logps']}, dict(ref_logps=x['ref'])
+    obj = L.DPOLoss(sft_weight=0.5)
+    clean = float(obj(inputs, outputs, **extra)['loss'])
+    real = getattr(obj, name)
+    twice = {'_seq_logps': lambda *a: (lambda r: (r[0], r[1], 2 * r[2]))(real(*a)), '_align_ref': lambda *a: 2 * real(*a), '_nll': lambda *a: 2 * real(*a)}[name]
+    monkeypatch.setattr(obj, name, twice)
+    changed = float(obj(inputs, outputs, **extra)['loss'])
+    on_cpu = float(obj({'labels': x['labels'].cpu()}, {'logps': x['logps'].cpu()}, ref_logps=x['ref'].cpu())['loss'])
+    assert abs(changed - clean) > 1e-3 and changed == pytest.approx(on_cpu, rel=1e-4)

@@ -30,6 +30,11 @@ class Loss:
         raise NotImplementedError
 
 
+def replaced(loss: Loss, names, defined) -> bool:
+    """Whether a method among ``names`` of ``loss`` is no longer the one that was defined: replaced on its class, or on the object."""
+    return any(n in vars(loss) or getattr(type(loss), n) is not f for n, f in zip(names, defined))
+
+
 def as_2d_labels(inputs: Dict[str, Any]) -> torch.Tensor:
     labels = inputs.get('labels')
     if labels is None:

@@ -5,7 +5,7 @@ hinge / ipo / kto_pair forms, label smoothing, ``sft_weight``,
 ``reference_free``; SimPO, CPO, ORPO.  Rows ``0::2`` are chosen and ``1::2``
 rejected, so a contiguous data-parallel slice of even length keeps pairs whole.
 On a GPU fp32 log-probs go through ``ops.preference_loss``; classes derived from
-these keep to the PyTorch forms.
+these and methods that were replaced on a class or an object keep to the PyTorch forms.
 """
 from __future__ import annotations
 
@@ -16,7 +16,7 @@ import torch.nn.functional as F
 
 from .. import ops
 from ..data_format import LossOutput
-from .base import Loss, as_2d_labels, token_logps
+from .base import Loss, as_2d_labels, replaced, token_logps
 
 
 class PreferenceLoss(Loss):
@@ -39,7 +39,7 @@ class PreferenceLoss(Loss):
         logps = outputs.get('logps')
         if logps is not None and logps.dim() == 1:
             logps = logps.unsqueeze(0)
-        if (type(self) not in _ON_KERNEL or logps is None or not logps.is_cuda or logps.dtype != torch.float32 or logps.shape != labels.shape or logps.numel() == 0
+        if (type(self) not in _ON_KERNEL or replaced(self, _METHODS, _DEFINED) or logps is None or not logps.is_cuda or logps.dtype != torch.float32 or logps.shape != labels.shape or logps.numel() == 0
                 or logps.shape[0] % 2):
             return None
         return labels.to(logps.device), logps
@@ -201,3 +201,5 @@ class ORPOLoss(PreferenceLoss):
 
 
 _ON_KERNEL = (DPOLoss, SimPOLoss, CPOLoss, ORPOLoss)
+_METHODS = ('_seq_logps', '_nll', '_align_ref')
+_DEFINED = tuple(getattr(PreferenceLoss, n) for n in _METHODS)

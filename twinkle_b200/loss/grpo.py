@@ -5,7 +5,8 @@ SAPO, CISPO, BNPO and DR-GRPO variants, including the alignment rules for
 ragged ``old_logps`` / ``ref_logps`` / ``advantages``.  Each variant here is a
 (ratio rule, surrogate rule, aggregation rule) triple on one class.  On a GPU the
 triple is computed by ``ops.policy_loss``; classes derived from these, whose rules
-may be others, and log-probs in other types than fp32 go through the methods.
+may be others, methods that were replaced on a class or an object, and log-probs in
+other types than fp32 go through the methods.
 """
 from __future__ import annotations
 
@@ -16,7 +17,7 @@ import torch
 
 from .. import ops
 from ..data_format import LossOutput
-from .base import Loss, as_2d_labels, token_logps
+from .base import Loss, as_2d_labels, replaced, token_logps
 
 
 def align_to_mask(values, mask: torch.Tensor, dtype=torch.float32) -> torch.Tensor:
@@ -75,7 +76,12 @@ def row_values(values, B: int, device) -> Optional[torch.Tensor]:
 
 
 class GRPOLoss(Loss):
-    rules: Dict[str, str] = dict(ratio='token', surrogate='clip', reduce='sequence')     # of ``ops.policy_loss``; a class has its own
+    rules: Dict[str, str] = dict(ratio='token', surrogate='clip', reduce='sequence')     # of ``ops.policy_loss``; a class has its own, which stand for its methods as they were defined
+    _said_by_rules = ('_log_ratio', '_surrogate', '_aggregate')
+
+    def __init_subclass__(cls, **kwargs):
+        super().__init_subclass__(**kwargs)
+        cls._defined = tuple(getattr(cls, n) for n in cls._said_by_rules)
 
     def __init__(self, epsilon: float = 0.2, epsilon_high: Optional[float] = None, beta: float = 0.0,
                  entropy_coef: float = 0.0, ignore_index: int = -100, **kwargs):
@@ -126,7 +132,7 @@ class GRPOLoss(Loss):
     # on the kernel ---------------------------------------------------------
     def _on_kernel(self, labels, logps, outputs) -> bool:
         ent = outputs.get('entropies')
-        return ('rules' in type(self).__dict__ and logps.is_cuda and logps.dtype == torch.float32 and logps.dim() == 2 and logps.shape == labels.shape and logps.numel() > 0
+        return ('rules' in type(self).__dict__ and not replaced(self, self._said_by_rules, self._defined) and logps.is_cuda and logps.dtype == torch.float32 and logps.dim() == 2 and logps.shape == labels.shape and logps.numel() > 0
                 and self.epsilon >= 0 and self.epsilon_high >= 0 and min((getattr(self, n, 1) for n in ('tau_pos', 'tau_neg', 'max_completion_length'))) > 0 and (self.entropy_coef <= 0.0 or (ent is not None and ent.shape == logps.shape)))
 
     def _kernel_loss(self, labels, logps, mask, outputs, old_logps, ref_logps, advantages, kwargs) -> torch.Tensor:
@@ -155,6 +161,9 @@ class GRPOLoss(Loss):
         low = ((ratio < 1 - self.epsilon) * m).sum() / n
         high = ((ratio > 1 + self.epsilon_high) * m).sum() / n
         return {'kl': float(kl.sum() / n), 'clip_low': float(low), 'clip_high': float(high)}
+
+
+GRPOLoss._defined = tuple(getattr(GRPOLoss, n) for n in GRPOLoss._said_by_rules)
 
 
 class GSPOLoss(GRPOLoss):
