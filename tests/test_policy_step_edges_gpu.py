@@ -142,3 +142,36 @@ def test_replaced_parts_of_a_preference_loss_are_followed(E, name, monkeypatch):
     changed = float(obj(inputs, outputs, **extra)['loss'])
     on_cpu = float(obj({'labels': x['labels'].cpu()}, {'logps': x['logps'].cpu()}, ref_logps=x['ref'].cpu())['loss'])
     assert abs(changed - clean) > 1e-3 and changed == pytest.approx(on_cpu, rel=1e-4)
+
+
+def _class_loss(name, x, logps, labels, **kwargs):
+    from twinkle_b200 import loss as L
+    extra = dict(old_logps=x['old'], advantages=[1.0, -0.5, 0.3, 2.0]) if name == 'GRPOLoss' else dict(ref_logps=x['ref'])
+    extra = {n: v.to(logps.device) if torch.is_tensor(v) else v for n, v in {**extra, **kwargs}.items()}
+    return getattr(L, name)()({'labels': labels}, {'logps': logps}, **extra)['loss']
+
+
+@pytest.mark.parametrize('name', ['GRPOLoss', 'DPOLoss', 'SimPOLoss'])
+def test_labels_may_be_written_again_before_the_backward_pass(E, name):  # noqa: F811
+    """A buffer that the next micro-batch fills, and one of inference mode."""
+    x = _policy_inputs(4, 50, 15)
+    lp = x['logps'].clone().requires_grad_()
+    want, = torch.autograd.grad(_class_loss(name, x, lp, x['labels'].clone()), lp)
+    labels = x['labels'].clone()
+    loss = _class_loss(name, x, lp, labels)
+    labels.fill_(-100)
+    assert torch.equal(torch.autograd.grad(loss, lp)[0], want)
+    with torch.inference_mode():
+        labels = x['labels'].clone()
+    assert torch.equal(torch.autograd.grad(_class_loss(name, x, lp, labels), lp)[0], want)
+
+
+@pytest.mark.parametrize('name', ['GRPOLoss', 'DPOLoss', 'ORPOLoss'])
+@pytest.mark.parametrize('dtype', [torch.bool, torch.int32, torch.float32])
+def test_labels_of_other_types_mean_what_they_mean_on_the_cpu(E, name, dtype):  # noqa: F811
+    """A truth value is no mask here: both differ from the index that is ignored."""
+    x = _policy_inputs(4, 50, 15)
+    x['labels'][2, 3] = 7
+    labels = (x['labels'] != -100) if dtype == torch.bool else x['labels'].to(dtype)
+    got = [float(_class_loss(name, x, x['logps'].to(d), labels.to(d))) for d in ('cuda', 'cpu')]
+    assert got[0] == pytest.approx(got[1], rel=1e-5)

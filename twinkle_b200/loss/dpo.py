@@ -34,7 +34,7 @@ class PreferenceLoss(Loss):
         return logps, mask, seq
 
     def _rows(self, inputs, outputs):
-        """Labels and log-probs where the kernel takes them, else None."""
+        """Mask (the labels may be written again before the backward pass) and log-probs where the kernel takes them, else None."""
         labels = as_2d_labels(inputs)
         logps = outputs.get('logps')
         if logps is not None and logps.dim() == 1:
@@ -42,7 +42,7 @@ class PreferenceLoss(Loss):
         if (type(self) not in _ON_KERNEL or replaced(self, _METHODS, _DEFINED) or logps is None or not logps.is_cuda or logps.dtype != torch.float32 or logps.shape != labels.shape or logps.numel() == 0
                 or logps.shape[0] % 2):
             return None
-        return labels.to(logps.device), logps
+        return (labels != self.ignore_index).to(logps.device), logps
 
     @staticmethod
     def _nll(chosen_seq_logps: torch.Tensor, mask: torch.Tensor) -> torch.Tensor:
@@ -126,7 +126,7 @@ class DPOLoss(PreferenceLoss):
         return LossOutput(loss=loss, num_tokens=0)
 
 
-    def _kernel_loss(self, labels, logps, ref, ref_chosen, ref_rejected) -> LossOutput:
+    def _kernel_loss(self, mask, logps, ref, ref_chosen, ref_rejected) -> LossOutput:
         if ref_chosen is not None and ref_rejected is not None:
             rc, rr = (torch.as_tensor(r).to(logps.device, logps.dtype).reshape(-1) for r in (ref_chosen, ref_rejected))
             pairs = logps.shape[0] // 2
@@ -142,8 +142,7 @@ class DPOLoss(PreferenceLoss):
                     ref = F.pad(ref, (0, logps.shape[1] - ref.shape[1]))
             elif not self.reference_free:
                 return LossOutput(loss=logps.sum() * 0.0, num_tokens=0)
-        loss, stats = ops.preference_loss(logps, labels, ref, self.loss_type, self.beta, label_smoothing=self.label_smoothing, nll_weight=max(self.sft_weight, 0.0),
-                                          ignore_index=self.ignore_index)
+        loss, stats = ops.preference_loss(logps, mask, ref, self.loss_type, self.beta, label_smoothing=self.label_smoothing, nll_weight=max(self.sft_weight, 0.0))
         self.last_stats = dict(zip(('rewards/chosen', 'rewards/rejected', 'rewards/margins', 'rewards/accuracies', 'logps/chosen', 'logps/rejected'), stats.tolist()))
         return LossOutput(loss=loss, num_tokens=0)
 
@@ -158,7 +157,7 @@ class SimPOLoss(PreferenceLoss):
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
         rows = self._rows(inputs, outputs)
         if rows is not None:
-            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='simpo', beta=self.beta, gamma=self.gamma, ignore_index=self.ignore_index)[0], num_tokens=0)
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='simpo', beta=self.beta, gamma=self.gamma)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         avg = seq / mask.sum(-1).clamp_min(1)
         z = self.beta * (avg[0::2] - avg[1::2]) - self.gamma
@@ -175,7 +174,7 @@ class CPOLoss(PreferenceLoss):
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
         rows = self._rows(inputs, outputs)
         if rows is not None:
-            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], beta=self.beta, nll_weight=self.bc_coef, ignore_index=self.ignore_index)[0], num_tokens=0)
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], beta=self.beta, nll_weight=self.bc_coef)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         pref = -F.logsigmoid(self.beta * (seq[0::2] - seq[1::2])).mean()
         return LossOutput(loss=pref + self.bc_coef * self._nll(seq[0::2], mask), num_tokens=0)
@@ -191,7 +190,7 @@ class ORPOLoss(PreferenceLoss):
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
         rows = self._rows(inputs, outputs)
         if rows is not None:
-            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='orpo', beta=self.lambda_orpo, nll_weight=1.0, ignore_index=self.ignore_index)[0], num_tokens=0)
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='orpo', beta=self.lambda_orpo, nll_weight=1.0)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         avg = seq / mask.sum(-1).clamp_min(1)
         c, r = avg[0::2], avg[1::2]

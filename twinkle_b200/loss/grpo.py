@@ -114,7 +114,7 @@ class GRPOLoss(Loss):
         if advantages is None:
             return LossOutput(loss=logps.sum() * 0.0, num_tokens=0)
         if self._on_kernel(labels, logps, outputs):
-            return LossOutput(loss=self._kernel_loss(labels.to(logps.device), logps, mask, outputs, old_logps, ref_logps, advantages, kwargs), num_tokens=0)
+            return LossOutput(loss=self._kernel_loss(logps, mask, outputs, old_logps, ref_logps, advantages, kwargs), num_tokens=0)
         old = logps.detach() if old_logps is None else align_to_mask(old_logps, mask, logps.dtype)
         adv = align_to_mask(advantages, mask, logps.dtype)
         ratio = torch.exp(self._log_ratio(logps, old, mask))
@@ -135,13 +135,13 @@ class GRPOLoss(Loss):
         return ('rules' in type(self).__dict__ and not replaced(self, self._said_by_rules, self._defined) and logps.is_cuda and logps.dtype == torch.float32 and logps.dim() == 2 and logps.shape == labels.shape and logps.numel() > 0
                 and self.epsilon >= 0 and self.epsilon_high >= 0 and min((getattr(self, n, 1) for n in ('tau_pos', 'tau_neg', 'max_completion_length'))) > 0 and (self.entropy_coef <= 0.0 or (ent is not None and ent.shape == logps.shape)))
 
-    def _kernel_loss(self, labels, logps, mask, outputs, old_logps, ref_logps, advantages, kwargs) -> torch.Tensor:
+    def _kernel_loss(self, logps, mask, outputs, old_logps, ref_logps, advantages, kwargs) -> torch.Tensor:
         grid = lambda v: None if v is None else align_to_mask(v, mask, logps.dtype)  # noqa: E731
         adv = row_values(advantages, logps.shape[0], logps.device)
         entropy_coef = max(self.entropy_coef, 0.0)
-        loss, stats = ops.policy_loss(logps, labels, grid(advantages) if adv is None else adv, grid(old_logps), grid(ref_logps) if self.beta > 0.0 else None,
+        loss, stats = ops.policy_loss(logps, mask, grid(advantages) if adv is None else adv, grid(old_logps), grid(ref_logps) if self.beta > 0.0 else None,
                                       outputs['entropies'] if entropy_coef else None, epsilon=self.epsilon, epsilon_high=self.epsilon_high, beta=self.beta, entropy_coef=entropy_coef,
-                                      ignore_index=self.ignore_index, **self.rules, **self._kernel_args(logps))
+                                      **self.rules, **self._kernel_args(logps))
         return self._kernel_reduced(loss, stats, kwargs)
 
     def _kernel_args(self, logps) -> Dict[str, Any]:
