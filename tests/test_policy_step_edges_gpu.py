@@ -175,3 +175,14 @@ def test_labels_of_other_types_mean_what_they_mean_on_the_cpu(E, name, dtype):  
     labels = (x['labels'] != -100) if dtype == torch.bool else x['labels'].to(dtype)
     got = [float(_class_loss(name, x, x['logps'].to(d), labels.to(d))) for d in ('cuda', 'cpu')]
     assert got[0] == pytest.approx(got[1], rel=1e-5)
+
+
+@pytest.mark.parametrize('shape', [(1, 50), (1, 30), (2, ), (4, 1), (4, 50)])
+@pytest.mark.parametrize('kind', ['sigmoid', 'ipo'])
+def test_references_for_several_rows_are_spread(E, shape, kind):  # noqa: F811
+    """One row of reference log-probs for all, two sums for all pairs."""
+    from twinkle_b200 import loss as L
+    x = _policy_inputs(4, 50, 15)
+    ref = torch.linspace(-2, -0.5, math.prod(shape)).view(shape)
+    got = [float(L.DPOLoss(loss_type=kind)({'labels': x['labels'].to(d)}, {'logps': x['logps'].to(d)}, ref_logps=ref)['loss']) for d in ('cuda', 'cpu')]
+    assert got[0] == pytest.approx(got[1], rel=1e-5)

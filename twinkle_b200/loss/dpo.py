@@ -86,8 +86,9 @@ class DPOLoss(PreferenceLoss):
         like the batch) or as the two sequence-level vectors ``ref_chosen_logps`` / ``ref_rejected_logps``
         (reference ``src/twinkle/loss/dpo.py:257-320``)."""
         rows = self._rows(inputs, outputs)
-        if rows is not None:
-            return self._kernel_loss(*rows, ref_outputs if ref_outputs is not None else ref_logps, ref_chosen_logps, ref_rejected_logps)
+        given = ref_outputs if ref_outputs is not None else ref_logps
+        if rows is not None and ((ref_chosen_logps is not None and ref_rejected_logps is not None) or self._row_by_row(given, rows[1])):
+            return self._kernel_loss(*rows, given, ref_chosen_logps, ref_rejected_logps)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         pc, pr = seq[0::2], seq[1::2]
         ref = None
@@ -97,7 +98,7 @@ class DPOLoss(PreferenceLoss):
             if rc.numel() != pc.numel() or rr.numel() != pr.numel():
                 raise ValueError(f'ref_chosen_logps / ref_rejected_logps must hold one value per pair ({pc.numel()}), got {rc.numel()} / {rr.numel()}')
         else:
-            ref = self._align_ref(ref_outputs if ref_outputs is not None else ref_logps, logps, mask)
+            ref = self._align_ref(given, logps, mask)
             if ref is None and not self.reference_free:
                 return LossOutput(loss=logps.sum() * 0.0, num_tokens=0)
             if ref is None:
@@ -125,6 +126,12 @@ class DPOLoss(PreferenceLoss):
         }
         return LossOutput(loss=loss, num_tokens=0)
 
+    @staticmethod
+    def _row_by_row(ref, logps) -> bool:
+        """Whether the reference has an entry per row (one that stands for several rows, or for all pairs, is spread by the PyTorch form)."""
+        if isinstance(ref, dict):
+            ref = ref.get('logps')
+        return ref is None or (torch.as_tensor(ref).dim() in (1, 2) and torch.as_tensor(ref).shape[0] == logps.shape[0])
 
     def _kernel_loss(self, mask, logps, ref, ref_chosen, ref_rejected) -> LossOutput:
         if ref_chosen is not None and ref_rejected is not None:
