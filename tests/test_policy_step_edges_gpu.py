@@ -186,3 +186,66 @@ def test_references_for_several_rows_are_spread(E, shape, kind):  # noqa: F811
     ref = torch.linspace(-2, -0.5, math.prod(shape)).view(shape)
     got = [float(L.DPOLoss(loss_type=kind)({'labels': x['labels'].to(d)}, {'logps': x['logps'].to(d)}, ref_logps=ref)['loss']) for d in ('cuda', 'cpu')]
     assert got[0] == pytest.approx(got[1], rel=1e-5)
+
+
+CLASSES = ['GRPOLoss', 'GSPOLoss', 'SAPOLoss', 'DPOLoss', 'SimPOLoss', 'CPOLoss', 'ORPOLoss']
+
+
+def _both(name, f):
+    """``f(loss as a function of log-probs, log-probs)`` of a class on the GPU in fp32 and on the CPU in fp64."""
+    from twinkle_b200 import loss as L
+    x = _policy_inputs(4, 50, 15)
+    x['labels'][2, 3] = 7
+    got = []
+    for device, dtype in (('cuda', torch.float32), ('cpu', torch.float64)):
+        y = {n: t.to(device) if n == 'labels' else t.to(device, dtype) for n, t in x.items()}
+        kw = dict(old_logps=y['old'], ref_logps=y['ref'], advantages=y['adv']) if issubclass(getattr(L, name), L.GRPOLoss) else dict(ref_logps=y['ref'])
+        obj = getattr(L, name)(**(dict(beta=0.1) if 'old_logps' in kw else {}))
+        got.append(f(lambda lp: obj({'labels': y['labels']}, {'logps': lp}, **kw)['loss'], y['logps'].clone()).double().cpu())
+    # sums of 50 terms in fp32, each off by a few roundings of 2^-24
+    assert torch.isfinite(got[0]).all() and (got[0] - got[1]).abs().max() <= 2**-17 * got[1].abs().max()
+    return got[0]
+
+
+@pytest.mark.parametrize('name', CLASSES)
+def test_gradients_of_gradients(E, name):  # noqa: F811
+    def second(f, lp):
+        lp.requires_grad_()
+        g, = torch.autograd.grad(3.0 * f(lp), lp, create_graph=True)
+        return torch.autograd.grad((g * torch.linspace(0, 1, g.numel(), device=g.device, dtype=g.dtype).view(g.shape)).square().sum(), lp)[0]
+
+    assert _both(name, second).abs().sum() > 0
+
+
+@pytest.mark.parametrize('name', CLASSES)
+def test_losses_in_functional_transforms(E, name):  # noqa: F811
+    _both(name, lambda f, lp: torch.func.grad(f)(lp))
+    _both(name, lambda f, lp: torch.func.jvp(f, (lp, ), (torch.ones_like(lp), ))[1])
+
+
+@pytest.mark.parametrize('name', CLASSES)
+def test_several_gradients_of_a_loss_at_once(E, name):  # noqa: F811
+    def batched(f, lp):
+        lp.requires_grad_()
+        return torch.autograd.grad(f(lp), lp, torch.tensor([1.0, -2.0, 0.5], device=lp.device, dtype=lp.dtype), is_grads_batched=True)[0]
+
+    _both(name, batched)
+
+
+def test_gradients_by_entropies_and_of_changed_inputs(E):  # noqa: F811
+    from twinkle_b200 import ops
+    x = _policy_inputs(4, 50, 15)
+    lp, en = x['logps'].clone().requires_grad_(), x['ent'].clone().requires_grad_()
+    call = lambda **k: ops.policy_loss(lp, x['labels'], x['adv'], x['old'], entropies=en, entropy_coef=0.1, **k)[0]  # noqa: E731
+    first = torch.autograd.grad(call(twice=True), (lp, en), create_graph=True)
+    plain = torch.autograd.grad(call(), (lp, en))
+    assert all((a - b).abs().max() <= 2**-20 * b.abs().max() for a, b in zip(first, plain)) and first[0].requires_grad
+    only, = torch.autograd.grad(call(twice=True), en, create_graph=True)
+    assert (only - plain[1]).abs().max() <= 2**-20 * plain[1].abs().max()
+    loss = call(twice=True)
+    x['old'].zero_()                       # what a first gradient does not need, a second would
+    assert torch.equal(torch.autograd.grad(loss, lp, retain_graph=True)[0], plain[0])
+    with pytest.raises(RuntimeError, match='inplace'):
+        torch.autograd.grad(loss, lp, create_graph=True)
+    with pytest.raises(RuntimeError, match='one gradient'):
+        torch.autograd.grad(call(), lp, torch.ones(2, device='cuda'), is_grads_batched=True)

@@ -5,7 +5,8 @@ hinge / ipo / kto_pair forms, label smoothing, ``sft_weight``,
 ``reference_free``; SimPO, CPO, ORPO.  Rows ``0::2`` are chosen and ``1::2``
 rejected, so a contiguous data-parallel slice of even length keeps pairs whole.
 On a GPU fp32 log-probs go through ``ops.preference_loss``; classes derived from
-these and methods that were replaced on a class or an object keep to the PyTorch forms.
+these, methods that were replaced on a class or an object, and functional transforms
+keep to the PyTorch forms.
 """
 from __future__ import annotations
 
@@ -39,7 +40,7 @@ class PreferenceLoss(Loss):
         logps = outputs.get('logps')
         if logps is not None and logps.dim() == 1:
             logps = logps.unsqueeze(0)
-        if (type(self) not in _ON_KERNEL or replaced(self, _METHODS, _DEFINED) or logps is None or not logps.is_cuda or logps.dtype != torch.float32 or logps.shape != labels.shape or logps.numel() == 0
+        if (type(self) not in _ON_KERNEL or replaced(self, _METHODS, _DEFINED) or ops.transformed() or logps is None or not logps.is_cuda or logps.dtype != torch.float32 or logps.shape != labels.shape or logps.numel() == 0
                 or logps.shape[0] % 2):
             return None
         return (labels != self.ignore_index).to(logps.device), logps
@@ -149,7 +150,8 @@ class DPOLoss(PreferenceLoss):
                     ref = F.pad(ref, (0, logps.shape[1] - ref.shape[1]))
             elif not self.reference_free:
                 return LossOutput(loss=logps.sum() * 0.0, num_tokens=0)
-        loss, stats = ops.preference_loss(logps, mask, ref, self.loss_type, self.beta, label_smoothing=self.label_smoothing, nll_weight=max(self.sft_weight, 0.0))
+        loss, stats = ops.preference_loss(logps, mask, ref, self.loss_type, self.beta, label_smoothing=self.label_smoothing, nll_weight=max(self.sft_weight, 0.0),
+                                          twice=True)
         self.last_stats = dict(zip(('rewards/chosen', 'rewards/rejected', 'rewards/margins', 'rewards/accuracies', 'logps/chosen', 'logps/rejected'), stats.tolist()))
         return LossOutput(loss=loss, num_tokens=0)
 
@@ -164,7 +166,7 @@ class SimPOLoss(PreferenceLoss):
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
         rows = self._rows(inputs, outputs)
         if rows is not None:
-            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='simpo', beta=self.beta, gamma=self.gamma)[0], num_tokens=0)
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='simpo', beta=self.beta, gamma=self.gamma, twice=True)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         avg = seq / mask.sum(-1).clamp_min(1)
         z = self.beta * (avg[0::2] - avg[1::2]) - self.gamma
@@ -181,7 +183,7 @@ class CPOLoss(PreferenceLoss):
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
         rows = self._rows(inputs, outputs)
         if rows is not None:
-            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], beta=self.beta, nll_weight=self.bc_coef)[0], num_tokens=0)
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], beta=self.beta, nll_weight=self.bc_coef, twice=True)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         pref = -F.logsigmoid(self.beta * (seq[0::2] - seq[1::2])).mean()
         return LossOutput(loss=pref + self.bc_coef * self._nll(seq[0::2], mask), num_tokens=0)
@@ -197,7 +199,7 @@ class ORPOLoss(PreferenceLoss):
     def __call__(self, inputs, outputs, **kwargs) -> LossOutput:
         rows = self._rows(inputs, outputs)
         if rows is not None:
-            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='orpo', beta=self.lambda_orpo, nll_weight=1.0)[0], num_tokens=0)
+            return LossOutput(loss=ops.preference_loss(rows[1], rows[0], form='orpo', beta=self.lambda_orpo, nll_weight=1.0, twice=True)[0], num_tokens=0)
         logps, mask, seq = self._seq_logps(inputs, outputs)
         avg = seq / mask.sum(-1).clamp_min(1)
         c, r = avg[0::2], avg[1::2]

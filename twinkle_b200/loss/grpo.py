@@ -5,8 +5,8 @@ SAPO, CISPO, BNPO and DR-GRPO variants, including the alignment rules for
 ragged ``old_logps`` / ``ref_logps`` / ``advantages``.  Each variant here is a
 (ratio rule, surrogate rule, aggregation rule) triple on one class.  On a GPU the
 triple is computed by ``ops.policy_loss``; classes derived from these, whose rules
-may be others, methods that were replaced on a class or an object, and log-probs in
-other types than fp32 go through the methods.
+may be others, methods that were replaced on a class or an object, functional transforms, and
+log-probs in other types than fp32 go through the methods.
 """
 from __future__ import annotations
 
@@ -132,7 +132,7 @@ class GRPOLoss(Loss):
     # on the kernel ---------------------------------------------------------
     def _on_kernel(self, labels, logps, outputs) -> bool:
         ent = outputs.get('entropies')
-        return ('rules' in type(self).__dict__ and not replaced(self, self._said_by_rules, self._defined) and logps.is_cuda and logps.dtype == torch.float32 and logps.dim() == 2 and logps.shape == labels.shape and logps.numel() > 0
+        return ('rules' in type(self).__dict__ and not replaced(self, self._said_by_rules, self._defined) and not ops.transformed() and logps.is_cuda and logps.dtype == torch.float32 and logps.dim() == 2 and logps.shape == labels.shape and logps.numel() > 0
                 and self.epsilon >= 0 and self.epsilon_high >= 0 and min((getattr(self, n, 1) for n in ('tau_pos', 'tau_neg', 'max_completion_length'))) > 0 and (self.entropy_coef <= 0.0 or (ent is not None and ent.shape == logps.shape)))
 
     def _kernel_loss(self, logps, mask, outputs, old_logps, ref_logps, advantages, kwargs) -> torch.Tensor:
@@ -141,7 +141,7 @@ class GRPOLoss(Loss):
         entropy_coef = max(self.entropy_coef, 0.0)
         loss, stats = ops.policy_loss(logps, mask, grid(advantages) if adv is None else adv, grid(old_logps), grid(ref_logps) if self.beta > 0.0 else None,
                                       outputs['entropies'] if entropy_coef else None, epsilon=self.epsilon, epsilon_high=self.epsilon_high, beta=self.beta, entropy_coef=entropy_coef,
-                                      **self.rules, **self._kernel_args(logps))
+                                      twice=True, **self.rules, **self._kernel_args(logps))
         return self._kernel_reduced(loss, stats, kwargs)
 
     def _kernel_args(self, logps) -> Dict[str, Any]:

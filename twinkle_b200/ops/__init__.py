@@ -1108,8 +1108,13 @@ def fused_linear_logprob(hidden, weight, labels, temperature: float = 1.0, with_
 
 
 # ------------------------------------------------------------------ losses
-_RATIO, _SURROGATE, _REDUCE = {'token': 0, 'sequence': 1}, {'clip': 0, 'soft': 1, 'weight': 2}, {'sequence': 0, 'token': 1, 'sum': 2}
-_PREFERENCE = ('sigmoid', 'hinge', 'ipo', 'kto_pair', 'simpo', 'orpo')
+_RATIO, _SURROGATE, _REDUCE = ({n: i for i, n in enumerate(names)} for names in (ref.RATIOS, ref.SURROGATES, ref.REDUCTIONS))
+_PREFERENCE = ref.PREFERENCES
+
+
+def transformed() -> bool:
+    """Whether a functional transform (``torch.func``) or forward-mode differentiation is under way: the loss kernels take part in neither."""
+    return torch._C._functorch.maybe_current_level() is not None or torch.autograd.forward_ad._current_level >= 0
 
 
 def _loss_rows(what: str, logps, labels, per_token, per_row):
@@ -1134,8 +1139,10 @@ def _side_by_side(t):
 
 
 def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entropies=None, ratio: str = 'token', surrogate: str = 'clip', reduce: str = 'sequence', epsilon: float = 0.2,
-                epsilon_high: Optional[float] = None, beta: float = 0.0, entropy_coef: float = 0.0, tau=(1.0, 1.0), denominator: float = 1.0, ignore_index: int = -100):
-    """``(loss, stats)`` of a policy step; differentiable by ``logps`` and ``entropies``.
+                epsilon_high: Optional[float] = None, beta: float = 0.0, entropy_coef: float = 0.0, tau=(1.0, 1.0), denominator: float = 1.0, ignore_index: int = -100,
+                twice: bool = False):
+    """``(loss, stats)`` of a policy step; differentiable by ``logps`` and ``entropies``, with ``twice`` as often as one likes: on a GPU the inputs are then kept, and the plain form gives a
+    gradient that is itself differentiated (without it such a call raises).
 
     ``logps [B, S]``; ``labels [B, S]``: tokens whose label is ``ignore_index`` (or a mask that is false) do not count; ``advantages`` per row ``[B]`` or per token; ``old_logps`` (the log-probs
     themselves when left out), ``ref_logps`` (used when ``beta`` is positive) and ``entropies`` (used with ``entropy_coef``) ``[B, S]``.  With ``l = clamp(logp − old, ±20)``, its mean over the row
@@ -1155,17 +1162,17 @@ def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entro
     entropies, ref_logps = entropies if entropy_coef else None, ref_logps if beta > 0 else None
     labels = _loss_rows('policy_loss', logps, labels, {'old_logps': old_logps, 'ref_logps': ref_logps, 'entropies': entropies}, {'advantages': advantages})
     constants = [t for t in (advantages, old_logps, ref_logps) if t is not None]
-    if _cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not (torch.is_grad_enabled() and any(t.requires_grad for t in constants)):
+    if _cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not transformed() and not (torch.is_grad_enabled() and any(t.requires_grad for t in constants)):
         loss, stats = ext().policy_loss(_side_by_side(logps), _side_by_side(entropies), _side_by_side(labels), _side_by_side(advantages), _side_by_side(old_logps), _side_by_side(ref_logps),
                                         *rules, epsilon, epsilon_high, beta, entropy_coef, *tau,
-                                        denominator, ignore_index)
+                                        denominator, ignore_index, twice)
         return loss, stats
     return ref.policy_loss(logps, labels, advantages, old_logps, ref_logps, entropies, ratio, surrogate, reduce, epsilon, epsilon_high, beta, entropy_coef, tau, denominator, ignore_index)
 
 
 def preference_loss(logps, labels, ref_logps=None, form: str = 'sigmoid', beta: float = 0.1, gamma: float = 0.0, label_smoothing: float = 0.0, nll_weight: float = 0.0,
-                    ignore_index: int = -100):
-    """``(loss, stats)`` of pairs of rows, chosen ``0::2`` and rejected ``1::2``; differentiable by ``logps [B, S]``.
+                    ignore_index: int = -100, twice: bool = False):
+    """``(loss, stats)`` of pairs of rows, chosen ``0::2`` and rejected ``1::2``; differentiable by ``logps [B, S]`` (``twice``: see ``policy_loss``).
 
     A row's level is the sum of its log-probs less that of ``ref_logps`` (``[B, S]``, or ``[B]`` summed already), for ``simpo`` and ``orpo`` their mean per token without a reference.  With
     ``z = beta (chosen − rejected) − gamma`` a pair costs ``−log σ(z)``, smoothed (``sigmoid``, ``simpo``), ``max(0, 1 − z)`` (``hinge``), ``(z − 1 / (2 beta))²`` (``ipo``), ``1 − σ(beta chosen) + σ(beta rejected)``
@@ -1180,9 +1187,9 @@ def preference_loss(logps, labels, ref_logps=None, form: str = 'sigmoid', beta: 
     if logps.shape[0] % 2:
         raise ValueError(f'preference_loss: rows in pairs, got {logps.shape[0]}')
     gamma, label_smoothing = (gamma if form in ('sigmoid', 'simpo', 'hinge', 'ipo') else 0.0), (label_smoothing if form in ('sigmoid', 'simpo') else 0.0)
-    if (_cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16)
+    if (_cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not transformed()
             and not (torch.is_grad_enabled() and ref_logps is not None and ref_logps.requires_grad)):
-        loss, stats = ext().preference_loss(_side_by_side(logps), _side_by_side(labels), _side_by_side(ref_logps), _PREFERENCE.index(form), beta, gamma, label_smoothing, nll_weight, ignore_index)
+        loss, stats = ext().preference_loss(_side_by_side(logps), _side_by_side(labels), _side_by_side(ref_logps), _PREFERENCE.index(form), beta, gamma, label_smoothing, nll_weight, ignore_index, twice)
         return loss, stats
     return ref.preference_loss(logps, labels, ref_logps, form, beta, gamma, label_smoothing, nll_weight, ignore_index)
 

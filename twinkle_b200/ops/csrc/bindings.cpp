@@ -74,8 +74,8 @@ void set_gemm_staged(int64_t);
 torch::Tensor paged_attn_shared(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t, int64_t, int64_t, int64_t, double);
 void cache_copy(const std::vector<torch::Tensor>&, const std::vector<int64_t>&, const std::vector<int64_t>&, const std::vector<int64_t>&);
 std::vector<torch::Tensor> policy_loss(const torch::Tensor&, const c10::optional<torch::Tensor>&, const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&,
-                                       const c10::optional<torch::Tensor>&, int64_t, int64_t, int64_t, double, double, double, double, double, double, double, int64_t);
-std::vector<torch::Tensor> preference_loss(const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&, int64_t, double, double, double, double, int64_t);
+                                       const c10::optional<torch::Tensor>&, int64_t, int64_t, int64_t, double, double, double, double, double, double, double, int64_t, bool);
+std::vector<torch::Tensor> preference_loss(const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&, int64_t, double, double, double, double, int64_t, bool);
 torch::Tensor grouped_gemm_wgrad(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t);
 std::vector<torch::Tensor> rmsnorm_fwd(const torch::Tensor&, const torch::Tensor&, double, double, const c10::optional<torch::Tensor>&);
 std::vector<torch::Tensor> rmsnorm_bwd(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, double,

@@ -501,6 +501,11 @@ def cache_copy(pools, src, dst, tokens=()) -> None:
             p[d, :n] = p[s, :n]
 
 
+# the kernels know these by their place
+RATIOS, SURROGATES, REDUCTIONS = ('token', 'sequence'), ('clip', 'soft', 'weight'), ('sequence', 'token', 'sum')
+PREFERENCES = ('sigmoid', 'hinge', 'ipo', 'kto_pair', 'simpo', 'orpo')
+
+
 def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entropies=None, ratio='token', surrogate='clip', reduce='sequence', epsilon=0.2, epsilon_high=None, beta=0.0,
                 entropy_coef=0.0, tau=(1.0, 1.0), denominator=1.0, ignore_index=-100):
     """See ``ops.policy_loss``; differentiable by everything."""
@@ -535,6 +540,25 @@ def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entro
         m = mask.to(logps.dtype)
         stats = torch.stack([((r - 1.0 - lr) * m).sum(), ((r < lo) * m).sum(), ((r > hi) * m).sum(), total]) / torch.stack([total.clamp_min(1.0)] * 3 + [torch.ones_like(total)])
     return loss, stats
+
+
+def policy_loss_gradient(up, wanted, logps, labels, advantages, old_logps, ref_logps, entropies, rules, numbers, ignore_index):
+    """``up`` times the derivatives of ``policy_loss`` by the tensors ``wanted``, differentiable where gradients are recorded.  ``rules`` are the numbers of ratio, surrogate and reduction in their
+    lists, ``numbers`` both bounds, beta, the entropies' weight, both temperatures and the denominator."""
+    low, high, beta, entropy, tau_pos, tau_neg, denominator = numbers
+    again = torch.is_grad_enabled()
+    with torch.enable_grad():
+        loss, _ = policy_loss(logps, labels, advantages, old_logps, ref_logps, entropies, RATIOS[rules[0]], SURROGATES[rules[1]], REDUCTIONS[rules[2]], low, high, beta, entropy,
+                              (tau_pos, tau_neg), denominator, ignore_index)
+        return torch.autograd.grad(loss, wanted, up.to(loss.dtype), create_graph=again)
+
+
+def preference_loss_gradient(up, wanted, logps, labels, ref_logps, form, numbers, ignore_index):
+    """Likewise of ``preference_loss``; ``numbers``: beta, gamma, label smoothing and the likelihood's weight."""
+    again = torch.is_grad_enabled()
+    with torch.enable_grad():
+        loss, _ = preference_loss(logps, labels, ref_logps, PREFERENCES[form], *numbers, ignore_index)
+        return torch.autograd.grad(loss, wanted, up.to(loss.dtype), create_graph=again)
 
 
 def preference_loss(logps, labels, ref_logps=None, form='sigmoid', beta=0.1, gamma=0.0, label_smoothing=0.0, nll_weight=0.0, ignore_index=-100):
