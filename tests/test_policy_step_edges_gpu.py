@@ -249,3 +249,16 @@ def test_gradients_by_entropies_and_of_changed_inputs(E):  # noqa: F811
         torch.autograd.grad(loss, lp, create_graph=True)
     with pytest.raises(RuntimeError, match='one gradient'):
         torch.autograd.grad(call(), lp, torch.ones(2, device='cuda'), is_grads_batched=True)
+
+
+@pytest.mark.parametrize('dtype', [torch.int64, torch.int32, torch.bool, torch.float64])
+def test_operands_of_other_types_are_converted(E, dtype):  # noqa: F811
+    from twinkle_b200 import ops
+    x = _policy_inputs(4, 50, 15)
+    adv, near = torch.tensor([[1], [0], [1], [1]], device='cuda'), (x['logps'] < -1).to(dtype)
+    args = dict(beta=0.1, entropy_coef=0.1)
+    want = ops.policy_loss(x['logps'], x['labels'], adv[:, 0].float(), near.float(), near.float(), near.float(), **args)
+    for a in (adv[:, 0], adv.expand(4, 50)):
+        got = ops.policy_loss(x['logps'], x['labels'], a.to(dtype), near, near, near, **args)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    assert torch.equal(ops.preference_loss(x['logps'], x['labels'], near)[0], ops.preference_loss(x['logps'], x['labels'], near.float())[0])

@@ -1130,11 +1130,11 @@ def _loss_rows(what: str, logps, labels, per_token, per_row):
     return labels if labels.dtype in (torch.bool, torch.int64) else labels.long()
 
 
-def _side_by_side(t):
-    """fp32 with the tokens of a row side by side (rows may be anywhere), on the kernels' terms."""
+def _side_by_side(t, labels: bool = False):
+    """fp32 (``labels`` as they are) with the tokens of a row side by side (rows may be anywhere), on the kernels' terms."""
     if t is None:
         return None
-    t = t if t.dtype in (torch.float32, torch.bool, torch.int64) else t.float()
+    t = t if labels or t.dtype == torch.float32 else t.float()
     return t if t.dim() == 1 or t.shape[1] <= 1 or t.stride(1) == 1 else t.contiguous()
 
 
@@ -1163,7 +1163,7 @@ def policy_loss(logps, labels, advantages, old_logps=None, ref_logps=None, entro
     labels = _loss_rows('policy_loss', logps, labels, {'old_logps': old_logps, 'ref_logps': ref_logps, 'entropies': entropies}, {'advantages': advantages})
     constants = [t for t in (advantages, old_logps, ref_logps) if t is not None]
     if _cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not transformed() and not (torch.is_grad_enabled() and any(t.requires_grad for t in constants)):
-        loss, stats = ext().policy_loss(_side_by_side(logps), _side_by_side(entropies), _side_by_side(labels), _side_by_side(advantages), _side_by_side(old_logps), _side_by_side(ref_logps),
+        loss, stats = ext().policy_loss(_side_by_side(logps), _side_by_side(entropies), _side_by_side(labels, True), _side_by_side(advantages), _side_by_side(old_logps), _side_by_side(ref_logps),
                                         *rules, epsilon, epsilon_high, beta, entropy_coef, *tau,
                                         denominator, ignore_index, twice)
         return loss, stats
@@ -1189,7 +1189,7 @@ def preference_loss(logps, labels, ref_logps=None, form: str = 'sigmoid', beta: 
     gamma, label_smoothing = (gamma if form in ('sigmoid', 'simpo', 'hinge', 'ipo') else 0.0), (label_smoothing if form in ('sigmoid', 'simpo') else 0.0)
     if (_cuda(logps) and logps.numel() and logps.shape[0] <= 65535 and logps.dtype in (torch.float32, torch.bfloat16, torch.float16) and not transformed()
             and not (torch.is_grad_enabled() and ref_logps is not None and ref_logps.requires_grad)):
-        loss, stats = ext().preference_loss(_side_by_side(logps), _side_by_side(labels), _side_by_side(ref_logps), _PREFERENCE.index(form), beta, gamma, label_smoothing, nll_weight, ignore_index, twice)
+        loss, stats = ext().preference_loss(_side_by_side(logps), _side_by_side(labels, True), _side_by_side(ref_logps), _PREFERENCE.index(form), beta, gamma, label_smoothing, nll_weight, ignore_index, twice)
         return loss, stats
     return ref.preference_loss(logps, labels, ref_logps, form, beta, gamma, label_smoothing, nll_weight, ignore_index)
 
