@@ -262,3 +262,52 @@ def test_operands_of_other_types_are_converted(E, dtype):  # noqa: F811
         got = ops.policy_loss(x['logps'], x['labels'], a.to(dtype), near, near, near, **args)
         assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.equal(ops.preference_loss(x['logps'], x['labels'], near)[0], ops.preference_loss(x['logps'], x['labels'], near.float())[0])
+
+
+# ------------------------------------------------------------- captured steps
+def _small(num_attention_heads=8, num_key_value_heads=2, **args):
+    from twinkle_b200.models import build_model, preset
+    from twinkle_b200.sampler.engine import NativeEngine
+    cfg = preset('qwen3-8b', num_hidden_layers=2, hidden_size=512, intermediate_size=1024, num_attention_heads=num_attention_heads, num_key_value_heads=num_key_value_heads, vocab_size=1024)
+    eng = NativeEngine(build_model(cfg, device='cuda', dtype=torch.bfloat16, seed=0), cfg, share_prompts=True, **args)
+    eng.share_from = 0
+    return eng
+
+
+def test_captured_steps_are_laid_out_as_eager_ones(E, monkeypatch):  # noqa: F811
+    """How many warps join a head and how far own pages are cut follow the plan and the table, not what was captured first; a shrinking group takes few captures."""
+    from twinkle_b200 import ops
+    from twinkle_b200.data_format import SamplingParams
+    real, seen = ops.paged_attention_shared, []
+
+    def noted(q, k, v, table, lens, prefix, scale=None):
+        room = prefix.own if getattr(prefix, 'own', -1) >= 0 else (table.shape[1] - prefix.shared) * prefix.block_size
+        seen.append((prefix.pieces > 8, min(8, (room + 255) // 256)))
+        return real(q, k, v, table, lens, prefix, scale)
+
+    monkeypatch.setattr(ops, 'paged_attention_shared', noted)
+    prompts = [[(7 * i + 3) % 900 for i in range(3000)], [(3 * i + 1) % 900 for i in range(2200)]]
+    laid, answers = [], []
+    for graphs in (True, False):
+        eng = _small(num_blocks=1000, block_size=16)
+        eng.use_cuda_graphs = graphs
+        seen.clear()
+        res = eng.generate(prompts, [SamplingParams(max_tokens=n, temperature=0.0, num_samples=3) for n in (9, 6)])
+        laid.append(set(seen))
+        answers.append([s.tokens for r in res for s in r.sequences])
+        assert bool(eng._graphs) == graphs
+    assert laid[0] == laid[1] and any(many for many, _ in laid[0]) and any(runs < 8 for _, runs in laid[0])
+    assert [a[:1] for a in answers[0]] == [a[:1] for a in answers[1]]
+
+
+def test_calls_with_other_plans_of_the_same_room(E):  # noqa: F811
+    """A plan with places that it does not use gives what the plan without them gives, bit for bit."""
+    from twinkle_b200 import ops
+    x, sizes, shared = batch([5, 2], [1500, 90], 30, 16, 16, 4, 128, seed=1, device='cuda')
+    plan, room = (ops.shared_prefix(sizes, shared, 16, 16, 4, items=n) for n in (0, 90))
+    assert room.items > plan.items
+    out = ops.paged_attention_shared(*x, plan)
+    assert torch.equal(out, ops.paged_attention_shared(*x, room))
+    wide = torch.cat([x[3], torch.zeros(7, 300, dtype=torch.int32, device='cuda')], 1)
+    own = (x[3].shape[1] - plan.shared) * 16
+    assert torch.equal(out, ops.paged_attention_shared(*x[:3], wide, x[4], room._replace(own=own)))

@@ -827,6 +827,7 @@ class SharedPrefix(NamedTuple):
     block_size: int
     shared: int               # fewest pages that a group which shares any shares
     pieces: int               # of a sequence's prefix, at most
+    own: int = -1             # tokens that most sequences have at most beside their prefix (−1: what the table has room for)
 
 
 def _prefix_items(sizes, blocks, block_size: int, group: int, kv_heads: int, sms: int):
@@ -876,14 +877,16 @@ def shared_prefix(sizes, blocks, block_size: int, heads: int, kv_heads: int, dev
         raise ValueError(f'shared_prefix: {heads} query heads on {kv_heads} key heads')
     work, lines = _prefix_items(sizes, blocks, block_size, heads // kv_heads, kv_heads, ext().num_sms() if torch.device(device).type == 'cuda' else 148)
     room = max(len(work), items)
-    flat = [x for w in work for x in w] + [0] * (8 * (room - len(work))) + [x for l in lines for x in l]
+    flat = [0] * (8 * (room - len(work))) + [x for w in work for x in w] + [x for l in lines for x in l]      # places that are not used come first: their CTAs leave before the others start
     return SharedPrefix(torch.tensor(flat, dtype=torch.int32).to(device), room, room, len(lines), heads, kv_heads, block_size, min((b for b in blocks if b), default=0),
                         max((l[2] for l in lines), default=0))
 
 
-def prefix_items(sequences: int, kv_heads: int, device='cuda') -> int:
-    """Pieces that the plan of any ``sequences`` fits."""
-    return sequences + 2 * (ext().num_sms() if torch.device(device).type == 'cuda' else 148) // kv_heads
+def prefix_items(sequences: int, kv_heads: int, device='cuda', group: int = 128) -> int:
+    """Pieces that the plan of any ``sequences`` fits; with ``group``, the query heads of a key head, of any whose groups that share pages have two sequences or more."""
+    per = 128 // group           # sequences of a tile: pairs need one for two, of two each groups of three need two
+    tiles = sequences if per == 1 else sequences * 2 // 3 if per == 2 else sequences // 2
+    return tiles + 2 * (ext().num_sms() if torch.device(device).type == 'cuda' else 148) // kv_heads
 
 
 def paged_attention_shared(q, k_cache, v_cache, block_tables, seq_lens, prefix: SharedPrefix, scale: Optional[float] = None):
@@ -900,7 +903,7 @@ def paged_attention_shared(q, k_cache, v_cache, block_tables, seq_lens, prefix: 
             and (q.data_ptr() | k_cache.data_ptr() | v_cache.data_ptr()) % 16 == 0):
         ints = (t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous() for t in (block_tables, seq_lens))
         return ext().paged_attn_shared(q.contiguous(), k_cache, v_cache, *ints, prefix.plan, prefix.items, prefix.slots, prefix.pieces,
-                                       max(block_tables.shape[1] - prefix.shared, 0) * prefix.block_size, scale)
+                                       prefix.own if prefix.own >= 0 else max(block_tables.shape[1] - prefix.shared, 0) * prefix.block_size, scale)
     return paged_attention_decode(q, k_cache, v_cache, block_tables, seq_lens, scale)
 
 

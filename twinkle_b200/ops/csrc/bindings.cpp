@@ -72,6 +72,7 @@ void set_gemm_pair(int64_t);
 void set_gemm_staged(int64_t);
 #ifndef TK_SERVING_ONLY
 torch::Tensor paged_attn_shared(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t, int64_t, int64_t, int64_t, double);
+std::tuple<int64_t, bool> paged_shared_split(int64_t, int64_t, int64_t, int64_t, int64_t);
 void cache_copy(const std::vector<torch::Tensor>&, const std::vector<int64_t>&, const std::vector<int64_t>&, const std::vector<int64_t>&);
 std::vector<torch::Tensor> policy_loss(const torch::Tensor&, const c10::optional<torch::Tensor>&, const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&,
                                        const c10::optional<torch::Tensor>&, int64_t, int64_t, int64_t, double, double, double, double, double, double, double, int64_t, bool);
@@ -199,6 +200,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("glu_columns", &tk::glu_columns, py::arg("p"), py::arg("gate"), py::arg("up"), py::arg("width"), py::arg("limit") = 0.0, py::arg("gelu") = false);
 #ifndef TK_SERVING_ONLY
   m.def("paged_attn_shared", &tk::paged_attn_shared);
+  m.def("paged_shared_split", &tk::paged_shared_split);
   m.def("cache_copy", &tk::cache_copy);
   m.def("policy_loss", &tk::policy_loss);
   m.def("preference_loss", &tk::preference_loss);

@@ -82,7 +82,7 @@ shared_prefix_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int* item = p.items + blockIdx.x * ITEM;
   const int row0 = item[0], seqs = item[1], tile0 = item[2], n = item[3], tokens = item[4], slot = item[5], named = item[6], kvh = blockIdx.y;
-  if (n <= 0) return;                      // an item that fills up a captured plan
+  if (n <= 0) return;                      // an item that fills up a plan (these come first: as the last of the grid they would keep the next kernel from starting beside the live ones)
   // not a plan for these sequences: rows beyond a slot, sequences, blocks or tokens that are not there (differences only: no sum of a plan's numbers wraps)
   if (seqs < 1 || seqs > ROWS / p.G || row0 < 0 || row0 > p.sequences - seqs || slot < 0 || slot >= p.slots || tokens < 1 || tokens > p.max_blocks * p.block_size || tile0 < 0 ||
       n > (tokens - 1) / BKV + 1 - tile0 || named < 0 || named > row0) {
@@ -699,6 +699,20 @@ static void launch_join(const SharedJoin& p, cudaStream_t stream) {
   launch_beside(shared_join_kernel<D, W>, dim3((p.total + HEADS - 1) / HEADS), sp::JOIN_WARPS * 32, 0, p, stream);
 }
 
+// How a call is laid out: CTAs of a sequence's own part, by what most have (where there is more a CTA's run is longer): 256 tokens each, more where that makes over 14 CTAs per SM; and whether
+// four warps join a head.  Heads with many pieces are summed by four: 13 sequences with 37 pieces of 32k tokens 35 -> 31 us; with 5 or fewer one warp does (64 sequences 55 against 57).
+static std::tuple<int64_t, bool> split_of(int64_t B, int64_t hq, int64_t hkv, int64_t pieces, int64_t room) {
+  const int64_t wide = B * hkv * ((hq / hkv + ow::HEADS - 1) / ow::HEADS);
+  int64_t runs = std::max<int64_t>(1, std::min<int64_t>(ow::RUNS, (room + ow::RUN * ow::TILE - 1) / (ow::RUN * ow::TILE)));
+  while (runs > 1 && wide * runs > 14 * num_sms()) runs = (runs + 1) / 2;
+  return {runs, pieces > 8};
+}
+// The same for whoever captures calls: captures of equal numbers are interchangeable.
+std::tuple<int64_t, bool> paged_shared_split(int64_t sequences, int64_t heads, int64_t kv_heads, int64_t pieces, int64_t room) {
+  TORCH_CHECK(sequences > 0 && kv_heads > 0 && heads > 0 && heads % kv_heads == 0, "sequences, heads of a multiple of the key heads");
+  return split_of(sequences, heads, kv_heads, pieces, room);
+}
+
 // One query token per sequence; pieces: slots of a sequence at most; room: tokens that most sequences have at most beside their prefix (what their split is chosen by); plan int32
 // [items · 8 + B · 4]: the items, then for every sequence the tokens of its prefix, its first slot, its slots and its row in them.
 torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& vc, const torch::Tensor& tables, const torch::Tensor& seq_lens, const torch::Tensor& plan,
@@ -716,10 +730,7 @@ torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc,
   TORCH_CHECK(reinterpret_cast<uintptr_t>(plan.data_ptr()) % 16 == 0 && tables.size(1) * bs < (int64_t(1) << 31), "plan on a 16-byte boundary, contexts below 2^31");
   c10::cuda::CUDAGuard guard(q.device());
   auto out = torch::empty_like(q);
-  // CTAs of a sequence's own part, by what most have (where there is more a CTA's run is longer): 256 tokens each, more where that makes over 14 CTAs per SM
-  const int64_t wide = B * hkv * ((G + ow::HEADS - 1) / ow::HEADS);
-  int64_t runs = std::max<int64_t>(1, std::min<int64_t>(ow::RUNS, (room + ow::RUN * ow::TILE - 1) / (ow::RUN * ow::TILE)));
-  while (runs > 1 && wide * runs > 14 * num_sms()) runs = (runs + 1) / 2;
+  const auto [runs, many] = split_of(B, hq, hkv, pieces, room);
   // one workspace: outputs of the pieces and of the runs, then their figures
   const int64_t pieces_rows = slots * hkv * sp::ROWS, runs_rows = runs * B * hq;
   auto work = torch::empty({(pieces_rows + runs_rows) * (D + 2)}, q.options().dtype(torch::kFloat32));
@@ -744,8 +755,6 @@ torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc,
   if (D == 128) launch_own<128>(own, stream); else launch_own<64>(own, stream);
   const SharedJoin join{rows, own.seq_lens, p.part, own.part, p.stat, own.stat, reinterpret_cast<bf16*>(out.data_ptr()), static_cast<int>(B * hq), static_cast<int>(hq), static_cast<int>(hkv),
                         static_cast<int>(G), static_cast<int>(slots), static_cast<int>(runs), static_cast<int>(tables.size(1) * bs)};
-  // heads with many pieces are summed by four warps: 13 sequences with 37 pieces of 32k tokens 35 -> 31 us; with 5 or fewer one warp does (64 sequences 55 against 57)
-  const bool many = pieces > 8;
   if (D == 128) many ? launch_join<128, 4>(join, stream) : launch_join<128, 1>(join, stream);
   else many ? launch_join<64, 4>(join, stream) : launch_join<64, 1>(join, stream);
   return out;

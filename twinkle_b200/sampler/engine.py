@@ -240,8 +240,8 @@ class NativeEngine:
             self._graphs.clear()          # captured steps hold the addresses of the pools
 
     def _shared(self, seqs: Sequence[_Seq], rows: int, captured: bool = False) -> Optional[ops.SharedPrefix]:
-        """The plan of a step whose sequences share prompts (None: nothing to share), filled up to ``rows`` sequences; ``captured``: with room for any plan of
-        that many."""
+        """The plan of a step whose sequences share prompts (None: nothing to share), filled up to ``rows`` sequences; ``captured``: with room for others in a
+        captured step."""
         if not self.share_prompts or self.cfg.layer_specs is not None or not any(s.origin is not None for s in seqs):
             return None
         sizes, blocks, last = [], [], None
@@ -259,9 +259,12 @@ class NativeEngine:
             return None
         key = (tuple(sizes), tuple(blocks), rows, captured)
         if self._plan[0] != key:
-            fill = rows - len(seqs)
-            self._plan = key, ops.shared_prefix(sizes + [1] * fill, blocks + [0] * fill, self.cache.block_size, heads, kv_heads, self.device,
-                                                ops.prefix_items(rows, kv_heads, self.device) if captured else 0)
+            sizes, blocks = sizes + [1] * (rows - len(seqs)), blocks + [0] * (rows - len(seqs))
+            plan = ops.shared_prefix(sizes, blocks, self.cache.block_size, heads, kv_heads, self.device)
+            if captured:      # room in steps, so that the plans of a shrinking batch take the same graphs; a call's workspace goes by it
+                room = min(ops.prefix_items(rows, kv_heads, self.device, heads // kv_heads), max(16, 1 << (plan.items - 1).bit_length()))
+                plan = ops.shared_prefix(sizes, blocks, self.cache.block_size, heads, kv_heads, self.device, room)
+            self._plan = key, plan
         return self._plan[1]
 
     def _heads(self) -> Tuple[int, int]:
@@ -395,11 +398,12 @@ class NativeEngine:
             x = self.model.norm(x)
         return self.model.logits(x).float()
 
-    def _graph_for(self, B: int, max_blocks: int, shared: bool = False):
-        """A captured decode step for batch bucket ``B`` and block-table width ``max_blocks`` (both powers of two); ``shared``: one that
-        reads shared prompts by a plan in static memory.
+    def _graph_for(self, B: int, max_blocks: int, prefix: Optional[ops.SharedPrefix] = None):
+        """A captured decode step for batch bucket ``B`` and block-table width ``max_blocks`` (both powers of two); with ``prefix`` one that reads shared prompts by a plan in static
+        memory, for plans of the same room that the kernels are laid out for alike.
         Inputs live in static tensors that ``decode_step`` fills before every replay; rows beyond the live batch have
         length 0 and write their K/V into block 0, which no sequence owns."""
+        shared = () if prefix is None else (prefix.items, *ops.ext().paged_shared_split(B, prefix.heads, prefix.kv_heads, prefix.pieces, prefix.own))
         key = (B, max_blocks, shared)
         ent = self._graphs.get(key)
         if ent is not None:
@@ -408,9 +412,8 @@ class NativeEngine:
         ints = torch.zeros(B * (max_blocks + 2), dtype=torch.int32, device=dev)       # filled by one copy per step
         st = {'tokens': torch.zeros(B, dtype=torch.long, device=dev), 'ints': ints, 'table': ints[:B * max_blocks].view(B, max_blocks),
               'seq_lens': ints[B * max_blocks:B * (max_blocks + 1)], 'slots': ints[B * (max_blocks + 1):], 'prefix': None, 'holds': None}
-        if shared:      # no piece of work yet; every plan of this batch fits
-            heads, kv_heads = self._heads()
-            st['prefix'] = ops.shared_prefix([1] * B, [0] * B, self.cache.block_size, heads, kv_heads, dev, ops.prefix_items(B, kv_heads, dev))
+        if prefix is not None:
+            st['prefix'], st['holds'] = prefix._replace(plan=prefix.plan.clone()), prefix.plan
 
         def body():
             # the token of a step is the last of its sequence; rows that fill up the batch have length 0 and position 0
@@ -445,8 +448,10 @@ class NativeEngine:
             Bb = 1 << max(B - 1, 0).bit_length()
             Mb = 1 << max(max_blocks - 1, 0).bit_length()
             prefix = self._shared(seqs, Bb, captured=True)
+            if prefix is not None:
+                prefix = prefix._replace(own=max(max_blocks - prefix.shared, 0) * self.cache.block_size)
             try:
-                st = self._graph_for(Bb, Mb, prefix is not None)
+                st = self._graph_for(Bb, Mb, prefix)
             except Exception as e:  # capture is an optimisation: the eager path below is always valid
                 self.use_cuda_graphs = False
                 import logging
@@ -457,9 +462,9 @@ class NativeEngine:
                 ints = torch.empty(Bb * (Mb + 2), dtype=torch.int32, pin_memory=True)
                 ops.ext().pack_step(ints, Bb, Mb, [s.blocks for s in seqs], [s.length for s in seqs], [s.state_slot for s in seqs])
                 st['ints'].copy_(ints, non_blocking=True)
-                if prefix is not None and st['holds'] is not prefix:
+                if prefix is not None and st['holds'] is not prefix.plan:
                     st['prefix'].plan.copy_(prefix.plan)
-                    st['holds'] = prefix
+                    st['holds'] = prefix.plan
                 if B < Bb:
                     st['tokens'].zero_()
                 st['tokens'][:B].copy_(last_tokens)
