@@ -311,3 +311,20 @@ def test_calls_with_other_plans_of_the_same_room(E):  # noqa: F811
     wide = torch.cat([x[3], torch.zeros(7, 300, dtype=torch.int32, device='cuda')], 1)
     own = (x[3].shape[1] - plan.shared) * 16
     assert torch.equal(out, ops.paged_attention_shared(*x[:3], wide, x[4], room._replace(own=own)))
+
+
+def test_steps_stay_captured_where_shared_ones_cannot_be(E, monkeypatch):  # noqa: F811
+    """A captured step over shared prompts that finds no memory costs the sharing, not the capture of plain steps."""
+    from twinkle_b200 import ops
+    from twinkle_b200.data_format import SamplingParams
+    prompts, params = [[(7 * i + 3) % 900 for i in range(400)]], [SamplingParams(max_tokens=6, temperature=0.0, num_samples=3)]
+    want = _small(num_blocks=200).generate(prompts, params)
+
+    def full(*args):
+        raise torch.cuda.OutOfMemoryError('no memory')
+
+    monkeypatch.setattr(ops, 'paged_attention_shared', full)
+    eng = _small(num_blocks=200)
+    res = eng.generate(prompts, params)
+    assert eng.use_cuda_graphs and eng._graphs and not any(k[2] for k in eng._graphs)
+    assert [s.tokens[:1] for s in res[0].sequences] == [s.tokens[:1] for s in want[0].sequences] and sorted(eng.cache.free) == list(range(1, 200))

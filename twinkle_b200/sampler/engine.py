@@ -185,6 +185,7 @@ class NativeEngine:
         # kernel (fewer than four query heads per key head).  us per layer, together / apart: 8 sequences of 512 tokens with 32/8 heads 12.1 / 15.2, of 256 11.7 / 8.7;
         # 4 of 512 with 16/8 heads 12.0 / 16.9, of 128 10.6 / 8.1
         self.share_from = 12288 if cfg.num_attention_heads < 4 * cfg.num_key_value_heads else 28672
+        self._share_captured = True            # until such a step could not be captured
         self._plan: Tuple[Any, Optional[ops.SharedPrefix]] = (None, None)      # of the last step with shared prompts
         self.device = device or next(model.parameters()).device
         self.dtype = next(model.parameters()).dtype
@@ -432,6 +433,15 @@ class NativeEngine:
         self._graphs[key] = st
         return st
 
+    def _captured(self, B: int, max_blocks: int, prefix: Optional[ops.SharedPrefix]):
+        """``_graph_for``, or None with a warning: capture is an optimisation, the eager path is always valid."""
+        try:
+            return self._graph_for(B, max_blocks, prefix)
+        except Exception as e:
+            import logging
+            logging.getLogger('twinkle_b200').warning(f'CUDA-graph capture of the decode step failed ({type(e).__name__}: {e}); running {"eagerly" if prefix is None else "without shared reading"}')
+            return None
+
     @torch.no_grad()
     def decode_step(self, seqs: List[_Seq], last_tokens: torch.Tensor) -> torch.Tensor:
         """One token for every sequence; returns logits ``[B, V]`` (fp32).  On a GPU the per-token work of a whole
@@ -447,16 +457,15 @@ class NativeEngine:
         if use_graph:
             Bb = 1 << max(B - 1, 0).bit_length()
             Mb = 1 << max(max_blocks - 1, 0).bit_length()
-            prefix = self._shared(seqs, Bb, captured=True)
+            prefix = self._shared(seqs, Bb, captured=True) if self._share_captured else None
             if prefix is not None:
                 prefix = prefix._replace(own=max(max_blocks - prefix.shared, 0) * self.cache.block_size)
-            try:
-                st = self._graph_for(Bb, Mb, prefix)
-            except Exception as e:  # capture is an optimisation: the eager path below is always valid
+            st = self._captured(Bb, Mb, prefix)
+            if st is None and prefix is not None:       # pages are then read per sequence
+                self._share_captured, prefix = False, None
+                st = self._captured(Bb, Mb, None)
+            if st is None:
                 self.use_cuda_graphs = False
-                import logging
-                logging.getLogger('twinkle_b200').warning(f'CUDA-graph capture of the decode step failed ({type(e).__name__}: {e}); running eagerly')
-                st = None
             if st is not None:
                 # a fresh pinned tensor each time: the allocator hands it out again only when the copy is done
                 ints = torch.empty(Bb * (Mb + 2), dtype=torch.int32, pin_memory=True)
