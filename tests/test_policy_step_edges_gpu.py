@@ -328,3 +328,50 @@ def test_steps_stay_captured_where_shared_ones_cannot_be(E, monkeypatch):  # noq
     res = eng.generate(prompts, params)
     assert eng.use_cuda_graphs and eng._graphs and not any(k[2] for k in eng._graphs)
     assert [s.tokens[:1] for s in res[0].sequences] == [s.tokens[:1] for s in want[0].sequences] and sorted(eng.cache.free) == list(range(1, 200))
+
+
+# --------------------------------------------------------------- long prefixes
+@pytest.mark.parametrize('sizes,prompts,bs,hq,hkv,D', [([3], [32760], 16, 8, 1, 128), ([2], [40000], 64, 4, 1, 64), ([2, 1, 3], [9000, 30, 7000], 16, 16, 2, 128)])
+def test_prefixes_of_many_pieces(E, sizes, prompts, bs, hq, hkv, D):  # noqa: F811
+    """Over 32 pieces a warp, over 128 a head, joined by four warps (the plan's own choice) and by one."""
+    from twinkle_b200 import ops
+    x, sizes, shared = batch(sizes, prompts, 40, bs, hq, hkv, D, device='cuda')
+    plan = ops.shared_prefix(sizes, shared, bs, hq, hkv)
+    assert plan.pieces > (32 if hkv > 1 else 100)
+    want = attention(*x)
+    for p in (plan, plan._replace(pieces=0)):
+        close(ops.paged_attention_shared(*x, p), *want)
+
+
+def test_a_prefix_in_pieces_of_one_block(E):  # noqa: F811
+    """160 pieces a head, more than any plan of this GPU has."""
+    from twinkle_b200 import ops
+    x, sizes, shared = batch([2], [160 * 128 + 5], 20, 16, 8, 1, 128, device='cuda')
+    items, lines = [[0, 2, i, 1, shared[0] * 16, i, 0, 0] for i in range(160)], [[shared[0] * 16, 0, 160, 8 * b] for b in range(2)]
+    numbers = torch.tensor([n for part in items + lines for n in part], dtype=torch.int32, device='cuda')
+    plan = ops.shared_prefix(sizes, shared, 16, 8, 1)._replace(plan=numbers, items=160, slots=160, pieces=160)
+    want = attention(*x)
+    for p in (plan, plan._replace(pieces=0)):
+        close(ops.paged_attention_shared(*x, p), *want)
+
+
+def test_captured_steps_behind_a_long_prompt(E):  # noqa: F811
+    """Captured and eager steps of a group behind 20k tokens, against sequences that read their pages for themselves."""
+    from twinkle_b200.sampler.engine import _Seq
+    from twinkle_b200.data_format import SamplingParams
+    prompt, steps = [(7 * i + 3) % 900 for i in range(20000)], {}
+    for how in ('captured', 'eager', 'apart'):
+        eng = _small(8, 1, num_blocks=1400)
+        eng.use_cuda_graphs, eng.share_prompts = how == 'captured', how != 'apart'
+        seqs = [_Seq(0, prompt, SamplingParams(max_tokens=8)) for _ in range(5)]
+        eng.prefill(seqs[:1])
+        eng.fork(seqs[0], seqs[1:])
+        steps[how] = []
+        for n in range(3):
+            for i, s in enumerate(seqs):
+                s.tokens.append((37 * n + 11 * i) % 900)
+            steps[how].append(eng.decode_step(seqs, torch.tensor([s.tokens[-1] for s in seqs], device='cuda')).clone())
+        eng.release(seqs)
+        assert bool(eng._graphs) == (how == 'captured')
+    for a, b, c in zip(*(steps[n] for n in ('captured', 'eager', 'apart'))):
+        assert (a - c).norm() / c.norm() < 2e-2 and (b - c).norm() / c.norm() < 2e-2
