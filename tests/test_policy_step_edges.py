@@ -20,3 +20,13 @@ def test_room_of_plans_of_groups():
         plan = ops.shared_prefix(sizes, blocks, bs, G * hkv, hkv, device='cpu', items=room)
         places = plan.plan[:8 * room].view(room, 8)
         assert plan.items == room and (places[:room - len(items), 3] == 0).all() and places[room - len(items):].tolist() == items
+
+
+def test_sharing_is_a_part_of_the_serving_subset():
+    from twinkle_b200.ops import build
+    names = lambda *parts: {p.rsplit('/', 1)[-1] for p in build._sources(parts)}  # noqa: E731
+    assert names('sharing') - names() == {'cache_copy.cu', 'paged_shared.cu'} and 'losses.cu' not in names(*build._PARTS)
+    with open(build._CSRC + '/bindings.cpp') as f:
+        text = f.read()
+    bound = text[text.index('TK_WITH_SHARING'):text.index('TK_WITH_CONVOLUTION')]
+    assert all(f'm.def("{n}"' in bound for n in ('paged_attn_shared', 'paged_shared_split', 'cache_copy'))

@@ -375,3 +375,11 @@ def test_captured_steps_behind_a_long_prompt(E):  # noqa: F811
         assert bool(eng._graphs) == (how == 'captured')
     for a, b, c in zip(*(steps[n] for n in ('captured', 'eager', 'apart'))):
         assert (a - c).norm() / c.norm() < 2e-2 and (b - c).norm() / c.norm() < 2e-2
+
+
+def test_sharing_on_a_subset_without_it_is_refused(E, monkeypatch):  # noqa: F811
+    from types import SimpleNamespace
+    from twinkle_b200 import ops
+    monkeypatch.setattr(ops, 'ext', lambda: SimpleNamespace())
+    with pytest.raises(RuntimeError, match='sharing'):
+        _small(num_blocks=20)

@@ -70,10 +70,10 @@ torch::Tensor mlstm_step(const torch::Tensor&, int64_t, int64_t, int64_t, int64_
                          const torch::Tensor&, const torch::Tensor&);
 void set_gemm_pair(int64_t);
 void set_gemm_staged(int64_t);
-#ifndef TK_SERVING_ONLY
 torch::Tensor paged_attn_shared(const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, const torch::Tensor&, int64_t, int64_t, int64_t, int64_t, double);
 std::tuple<int64_t, bool> paged_shared_split(int64_t, int64_t, int64_t, int64_t, int64_t);
 void cache_copy(const std::vector<torch::Tensor>&, const std::vector<int64_t>&, const std::vector<int64_t>&, const std::vector<int64_t>&);
+#ifndef TK_SERVING_ONLY
 std::vector<torch::Tensor> policy_loss(const torch::Tensor&, const c10::optional<torch::Tensor>&, const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&,
                                        const c10::optional<torch::Tensor>&, int64_t, int64_t, int64_t, double, double, double, double, double, double, double, int64_t, bool);
 std::vector<torch::Tensor> preference_loss(const torch::Tensor&, const torch::Tensor&, const c10::optional<torch::Tensor>&, int64_t, double, double, double, double, int64_t, bool);
@@ -149,6 +149,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("attention_packed", &tk::attention_packed, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("cu"), py::arg("max_seqlen"), py::arg("scale"),
         py::arg("sinks") = py::none(), py::arg("gate") = py::none(), py::arg("window") = 0, py::arg("chunk") = 0, py::arg("cap") = 0.0, py::arg("temp") = py::none(), py::arg("slope") = py::none(),
         py::arg("rate") = py::none(), py::arg("table") = py::none(), py::arg("bucket") = py::none());
+#ifdef TK_WITH_SHARING
+  m.def("paged_attn_shared", &tk::paged_attn_shared);
+  m.def("paged_shared_split", &tk::paged_shared_split);
+  m.def("cache_copy", &tk::cache_copy);
+#endif
 #ifdef TK_WITH_CONVOLUTION
   m.def("conv_heads", &tk::conv_heads, py::arg("proj"), py::arg("weight"), py::arg("pos"), py::arg("hq"), py::arg("hkv"), py::arg("d"), py::arg("e"), py::arg("eps"),
         py::arg("coef") = 0.0, py::arg("every") = 0, py::arg("v_first") = py::none(), py::arg("lam") = py::none(), py::arg("step") = false,
@@ -199,9 +204,6 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
         py::arg("out") = py::none(), py::arg("accumulate") = false, py::arg("x2") = py::none(), py::arg("w2") = py::none(), py::arg("act") = py::none());
   m.def("glu_columns", &tk::glu_columns, py::arg("p"), py::arg("gate"), py::arg("up"), py::arg("width"), py::arg("limit") = 0.0, py::arg("gelu") = false);
 #ifndef TK_SERVING_ONLY
-  m.def("paged_attn_shared", &tk::paged_attn_shared);
-  m.def("paged_shared_split", &tk::paged_shared_split);
-  m.def("cache_copy", &tk::cache_copy);
   m.def("policy_loss", &tk::policy_loss);
   m.def("preference_loss", &tk::preference_loss);
   m.def("grouped_gemm_wgrad", &tk::grouped_gemm_wgrad);

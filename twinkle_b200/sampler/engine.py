@@ -188,6 +188,8 @@ class NativeEngine:
         self._share_captured = True            # until such a step could not be captured
         self._plan: Tuple[Any, Optional[ops.SharedPrefix]] = (None, None)      # of the last step with shared prompts
         self.device = device or next(model.parameters()).device
+        if share_prompts and self.device.type == 'cuda' and not hasattr(ops.ext(), 'cache_copy'):
+            raise RuntimeError("share_prompts: this process runs on a serving subset without the part 'sharing' (ops.build.prefer_serving)")
         self.dtype = next(model.parameters()).dtype
         if num_blocks is None:
             elem = 2 if self.dtype != torch.float32 else 4
