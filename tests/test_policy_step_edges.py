@@ -30,3 +30,63 @@ def test_sharing_is_a_part_of_the_serving_subset():
         text = f.read()
     bound = text[text.index('TK_WITH_SHARING'):text.index('TK_WITH_CONVOLUTION')]
     assert all(f'm.def("{n}"' in bound for n in ('paged_attn_shared', 'paged_shared_split', 'cache_copy'))
+
+
+def _engine_and(stack, n, **args):
+    from twinkle_b200.data_format import SamplingParams
+    from twinkle_b200.models import build_model, preset
+    from twinkle_b200.sampler.engine import NativeEngine, _Seq
+    cfg = preset(stack)
+    eng = NativeEngine(build_model(cfg, device='cpu', dtype=torch.float32, seed=0), cfg, share_prompts=True, **{**dict(num_blocks=64, block_size=4, max_batch=8), **args})
+    return eng, [_Seq(0, [3, 4, 5, 6, 7, 8], SamplingParams(max_tokens=4)) for _ in range(n)]
+
+
+@pytest.mark.parametrize('what', ['has not run', 'other prompt', 'longer prompt', 'other adapter', 'has run', 'has tokens'])
+def test_forks_that_are_refused(what):
+    eng, (a, b, c) = _engine_and('tiny-dense', 3)
+    if what != 'has not run':
+        eng.prefill([a])
+    if what == 'other prompt':
+        b.prompt = [9] * 6
+    elif what == 'longer prompt':
+        b.prompt = a.prompt + [1]
+    elif what == 'other adapter':
+        b.slot = 1
+    elif what == 'has run':
+        eng.prefill([b])
+    elif what == 'has tokens':
+        b.tokens.append(1)
+    free, held = list(eng.cache.free), list(b.blocks)
+    with pytest.raises(ValueError):
+        eng.fork(a, [c, b])
+    assert eng.cache.free == free and not eng.cache.sharers and b.blocks == held and c.blocks == [] and a.origin is None
+
+
+@pytest.mark.parametrize('stack', ['tiny-dense', 'tiny-hybrid'])
+def test_forks_of_a_sequence_that_has_gone_on(stack):
+    """Keys and values of the prompt are still there; a state is not."""
+    eng, (a, b, c) = _engine_and(stack, 3)
+    eng.prefill([a])
+    a.tokens.append(11)
+    eng.grow([a])
+    eng.decode_step([a], torch.tensor([11]))
+    if stack == 'tiny-hybrid':
+        with pytest.raises(ValueError, match='state'):
+            eng.fork(a, [b])
+        return
+    eng.fork(a, [b])
+    eng.prefill([c])
+    for s in (b, c):
+        s.tokens.append(12)
+        eng.grow([s])
+    x, y = (eng.decode_step([s], torch.tensor([12])) for s in (b, c))
+    assert torch.allclose(x, y, atol=1e-5)
+
+
+def test_routing_of_forks_is_that_of_the_prompt():
+    eng, (a, b) = _engine_and('tiny-dense', 2)
+    eng.prefill([a])
+    a.routed = [torch.arange(9).view(9, 1)]
+    a.tokens += [1, 2, 3]
+    eng.fork(a, [b])
+    assert b.routed[0].tolist() == [[i] for i in range(6)]

@@ -225,12 +225,19 @@ class NativeEngine:
             s.state_slot = self.cache.allocate_slot()
 
     def fork(self, origin: _Seq, seqs: Sequence[_Seq]) -> None:
-        """Let ``seqs`` continue the prompt of ``origin``, which has run: its full blocks are shared, the rest and the state are copied."""
+        """Let ``seqs`` continue the prompt of ``origin``, which has run: its full blocks are shared, the rest and the state are copied (a state that has gone beyond the prompt cannot be)."""
+        who = lambda s: (s.prompt, s.slot, s.lora_rank, s.lora_scale, s.lora_target)  # noqa: E731
+        if not origin.blocks or any(who(s) != who(origin) or s.blocks or s.tokens for s in seqs):
+            raise ValueError('fork: a sequence that has run, and others that have not, with its prompt and adapter')
+        if origin.tokens and (origin.state_slot or origin.linear):
+            raise ValueError(f'fork: the state of the sequence has seen {len(origin.tokens)} tokens behind its prompt')
+        if self.cache.num_slots and len(seqs) > len(self.cache.free_slots):
+            raise RuntimeError(f'per-sequence state exhausted: {len(seqs)} forks, {len(self.cache.free_slots)} slots')
         lists, copies = self.cache.fork(origin.blocks, len(origin.prompt), [self.cache.blocks_for(len(s.prompt) + (s.params.max_tokens or 0) + 1) for s in seqs])
         slots = []
         for s, blocks in zip(seqs, lists):
             s.blocks, s.state_slot, s.origin = blocks, self.cache.allocate_slot(), origin
-            s.linear, s.rope_delta, s.routed = dict(origin.linear), origin.rope_delta, None if origin.routed is None else list(origin.routed)
+            s.linear, s.rope_delta, s.routed = dict(origin.linear), origin.rope_delta, None if origin.routed is None else [r[:len(origin.prompt)] for r in origin.routed]
             if s.state_slot:
                 slots.append((origin.state_slot, s.state_slot))
         origin.origin = origin
