@@ -90,3 +90,39 @@ def test_routing_of_forks_is_that_of_the_prompt():
     a.tokens += [1, 2, 3]
     eng.fork(a, [b])
     assert b.routed[0].tolist() == [[i] for i in range(6)]
+
+
+# heads, groups, shared tokens, own tokens, and what a layer of a captured step took on a B200: us together, us apart
+MEASURED = [((32, 4, 128), [8], [1024], [256] * 8, 11.2, 9.1), ((32, 4, 128), [16], [1024], [256] * 16, 12.5, 17.4), ((32, 8, 64), [8] * 8, [64] * 8, [256] * 64, 17.3, 11.3),
+            ((32, 8, 64), [64], [1024], [256] * 64, 19.9, 24.6), ((32, 8, 128), [64], [512], [256] * 64, 23.3, 35.0), ((12, 2, 128), [4], [512], [256] * 4, 9.7, 6.4),
+            ((32, 8, 128), [4], [512], [256] * 4, 9.6, 7.6), ((32, 8, 128), [8], [512], [256] * 8, 10.4, 15.1), ((16, 8, 128), [2], [512], [256] * 2, 9.4, 18.7), ((8, 8, 128), [4], [1024], [256] * 4, 10.7, 33.3),
+            ((16, 8, 128), [4], [496], [256] * 4, 9.6, 21.9), ((32, 8, 128), [2] + [1] * 62, [4096] + [0] * 62, [256] * 2 + [4352] * 62, 195.0, 167.2), ((32, 8, 64), [2] * 32, [512] * 32, [256] * 64, 30.2, 18.2),
+            ((32, 8, 128), [2] * 32, [128] * 32, [256] * 64, 30.3, 24.5), ((32, 8, 128), [256], [1024], [256] * 256, 68.1, 119.1), ((12, 2, 128), [64], [128], [256] * 64, 11.6, 16.5)]
+
+
+@pytest.mark.parametrize('heads,sizes,tokens,own,together,apart', MEASURED)
+def test_the_faster_way_is_expected_to_be(heads, sizes, tokens, own, together, apart):
+    a, b = ops.shared_times(sizes, [t // 16 for t in tokens], own, 16, *heads, device='cpu')
+    assert (a < b) == (together < apart)
+
+
+@pytest.mark.parametrize('heads,sizes,tokens,own,together,apart', MEASURED)
+def test_an_engine_shares_where_it_pays(heads, sizes, tokens, own, together, apart):
+    """By the groups and the lengths of its sequences; 0 for wherever pages are shared; never for a cache that the kernel does not take."""
+    from twinkle_b200.data_format import SamplingParams
+    from twinkle_b200.models import build_model, preset
+    from twinkle_b200.sampler.engine import NativeEngine, _Seq
+    cfg = preset('qwen3-8b', num_hidden_layers=1, hidden_size=64, intermediate_size=64, num_attention_heads=heads[0], num_key_value_heads=heads[1], head_dim=heads[2], vocab_size=64)
+    eng = NativeEngine(build_model(cfg, device='cpu', dtype=torch.bfloat16, seed=0), cfg, num_blocks=4, share_prompts=True)
+    seqs, at = [], 0
+    for n, t in zip(sizes, tokens):
+        group = [_Seq(0, [1] * (t or own[at + i] - 1), SamplingParams(), tokens=[1] * (own[at + i] if t else 1)) for i in range(n)]
+        for s in group:
+            s.origin, s.blocks = group[0] if n > 1 else None, [1] * ((s.length + 271) // 16)
+        seqs += group
+        at += n
+    assert (eng._shared(seqs, len(seqs)) is not None) == (together < apart)
+    eng.share_from = 0
+    assert eng._shared(seqs, len(seqs)) is not None
+    eng.share_from, eng.dtype = 1.0, torch.float32
+    assert eng._shared(seqs, len(seqs)) is None

@@ -889,6 +889,35 @@ def prefix_items(sequences: int, kv_heads: int, device='cuda', group: int = 128)
     return tiles + 2 * (ext().num_sms() if torch.device(device).type == 'cuda' else 148) // kv_heads
 
 
+def shared_times(sizes, blocks, own, block_size: int, heads: int, kv_heads: int, width: int, room: int = 1 << 20, device='cuda') -> Tuple[float, float]:
+    """What a layer's decode is expected to take, in us: ``(paged_attention_shared, paged_attention_decode)`` for groups as in ``shared_prefix`` whose sequences have ``own`` tokens beside
+    their prefix, in a table with ``room`` for so many tokens.
+
+    Shared: 2.5 us per block of 128 tokens on an SM, a piece's start and end as two of them; a run of own tokens; all own tokens. Apart: waves of two CTAs per SM, the longest CTA's share of its
+    sequence (clusters as ``paged_decode.cu`` sizes them), all tokens; on the vector kernel (fewer than four query heads per key head) the longest sequence and all tokens. The rates are fitted to
+    captured steps of 2802 batches (2 to 256 sequences in groups of 1 to 256 behind 32 to 11k tokens, 12/2 to 64/8 heads of 64 and 128, B200). Of 757 others they name the slower way by more than 5 % in
+    38, 8 of these sharing (at most 1.5 times as slow); a bound on the tokens that are not read again (28k, or 12k, times key heads) did in 137 and 51 (up to 2.6 times as slow)."""
+    sms = ext().num_sms() if torch.device(device).type == 'cuda' else 148
+    group = heads // kv_heads
+    items, _ = _prefix_items(sizes, blocks, block_size, group, kv_heads, sms)
+    shared = [b * block_size for n, b in zip(sizes, blocks) for _ in range(n)]
+    token, ctas, longest = 1e-3 * kv_heads * width / 128, len(own) * kv_heads * ((group + 7) // 8), max(map(sum, zip(shared, own)))
+    runs = max(1, min(8, (max(own) + 255) // 256))
+    while runs > 1 and ctas * runs > 14 * sms:
+        runs = (runs + 1) // 2
+    chain = max((max(i[3] for i in items) + 2, sum(i[3] + 2 for i in items) * kv_heads / sms)) if items else 0.0
+    together = 2.5 + 2.5 * chain + 6.4e-3 * max(own) / runs + 0.091 * token * sum(own)
+    if group < 4:
+        return together, 2.2 + 0.021 * longest + 0.093 * token * (sum(shared) + sum(own))
+    cut = 1
+    while cut < 8 and 4 * ctas * cut < 7 * sms and 2 * cut <= room // 64:
+        cut *= 2
+    waves = (ctas * cut + 2 * sms - 1) // (2 * sms)
+    if width == 128:
+        return together, 6.1 * waves + 9.2e-3 * longest / cut + 0.049 * token * (sum(shared) + sum(own))
+    return together, 4.1 + 0.8 * waves + 8e-3 * longest / cut + 0.034 * token * (sum(shared) + sum(own))
+
+
 def paged_attention_shared(q, k_cache, v_cache, block_tables, seq_lens, prefix: SharedPrefix, scale: Optional[float] = None):
     """``paged_attention_decode`` for sequences that share pages: the shared ones are read once per group.  The shared ones are those that the
     table row of a group's first sequence names, whose length may be anything; a sequence that is shorter than what its group shares (0: a finished one) attends to its own length of its own row.  A page outside the pools counts as zeros and sets the error word.

@@ -181,10 +181,8 @@ class NativeEngine:
         """``share_prompts``: sequences with the same prompt (the samples of a request, repeated prompts) run through it once, share its full cache
         blocks and read them once per step.  Results then differ by the rounding of other tile shapes and orders of sums."""
         self.model, self.cfg, self.share_prompts = model, cfg, share_prompts
-        # Reading shared pages once takes two more launches: it pays from about 28k keys (times key heads) that are not read again, 12k where a step without it decodes on the vector
-        # kernel (fewer than four query heads per key head).  us per layer, together / apart: 8 sequences of 512 tokens with 32/8 heads 12.1 / 15.2, of 256 11.7 / 8.7;
-        # 4 of 512 with 16/8 heads 12.0 / 16.9, of 128 10.6 / 8.1
-        self.share_from = 12288 if cfg.num_attention_heads < 4 * cfg.num_key_value_heads else 28672
+        # Shared pages are read once per step where that is expected to take this much less time than reading them per sequence (``ops.shared_times``); 0: wherever there are any
+        self.share_from = 1.0
         self._share_captured = True            # until such a step could not be captured
         self._plan: Tuple[Any, Optional[ops.SharedPrefix]] = (None, None)      # of the last step with shared prompts
         self.device = device or next(model.parameters()).device
@@ -264,18 +262,28 @@ class NativeEngine:
             last = s.origin
         blocks = [b if n > 1 else 0 for n, b in zip(sizes, blocks)]
         heads, kv_heads = self._heads()
-        again = sum((n - 1) * b for n, b in zip(sizes, blocks)) * self.cache.block_size * kv_heads
-        if again == 0 or again < self.share_from:
+        if not any(blocks):
             return None
-        key = (tuple(sizes), tuple(blocks), rows, captured)
+        key = (tuple(sizes), tuple(blocks), rows, captured, self.share_from, seqs[0].length >> 8)      # which way is faster changes with the answers' lengths, but slowly
         if self._plan[0] != key:
-            sizes, blocks = sizes + [1] * (rows - len(seqs)), blocks + [0] * (rows - len(seqs))
-            plan = ops.shared_prefix(sizes, blocks, self.cache.block_size, heads, kv_heads, self.device)
-            if captured:      # room in steps, so that the plans of a shrinking batch take the same graphs; a call's workspace goes by it
-                room = min(ops.prefix_items(rows, kv_heads, self.device, heads // kv_heads), max(16, 1 << (plan.items - 1).bit_length()))
-                plan = ops.shared_prefix(sizes, blocks, self.cache.block_size, heads, kv_heads, self.device, room)
+            bs, plan = self.cache.block_size, None
+            own = [s.length - b * bs for s, b in zip(seqs, (b for n, b in zip(sizes, blocks) for _ in range(n)))]
+            if not self.share_from or self._pays(sizes, blocks, own, bs << max(max(len(s.blocks) for s in seqs) - 1, 0).bit_length()):
+                sizes, blocks = sizes + [1] * (rows - len(seqs)), blocks + [0] * (rows - len(seqs))
+                plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device)
+                if captured:      # room in steps, so that the plans of a shrinking batch take the same graphs; a call's workspace goes by it
+                    room = min(ops.prefix_items(rows, kv_heads, self.device, heads // kv_heads), max(16, 1 << (plan.items - 1).bit_length()))
+                    plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device, room)
             self._plan = key, plan
         return self._plan[1]
+
+    def _pays(self, sizes: Sequence[int], blocks: Sequence[int], own: Sequence[int], room: int) -> bool:
+        """Whether a step of these groups is expected to be faster with shared pages read once; never where the kernel does not take the cache."""
+        (heads, kv_heads), (_, width, value) = self._heads(), self.cfg.kv_layout()[0]
+        if self.dtype != torch.bfloat16 or width not in (64, 128) or value != width or self.cache.block_size % 8:
+            return False
+        together, apart = ops.shared_times(sizes, blocks, own, self.cache.block_size, heads, kv_heads, width, room, self.device)
+        return apart > self.share_from * together
 
     def _heads(self) -> Tuple[int, int]:
         return self.cfg.num_attention_heads, self.cfg.kv_layout()[0][0]
