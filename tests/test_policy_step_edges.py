@@ -126,3 +126,14 @@ def test_an_engine_shares_where_it_pays(heads, sizes, tokens, own, together, apa
     assert eng._shared(seqs, len(seqs)) is not None
     eng.share_from, eng.dtype = 1.0, torch.float32
     assert eng._shared(seqs, len(seqs)) is None
+
+
+def test_own_pages_are_cut_by_the_longest_own_part():
+    """Not by what the widest row of the table leaves beside the shortest prefix: a sequence that shares nothing is its own part from its first token."""
+    eng, seqs = _engine_and('tiny-dense', 5, num_blocks=2000, block_size=8)
+    eng.share_from = 0
+    for s, prompt, room in zip(seqs, (800, 800, 800, 400, 40), (10, 10, 12, 60, 6)):
+        s.prompt, s.blocks = [1] * prompt, [1] * (prompt // 8 + room)
+    for s in seqs[:3]:
+        s.origin = seqs[0]
+    assert eng._shared(seqs, 5).own == 8 * (50 + 60) and eng._shared(seqs[:3], 3).own == 8 * 12

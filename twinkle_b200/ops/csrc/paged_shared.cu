@@ -699,7 +699,7 @@ static void launch_join(const SharedJoin& p, cudaStream_t stream) {
   launch_beside(shared_join_kernel<D, W>, dim3((p.total + HEADS - 1) / HEADS), sp::JOIN_WARPS * 32, 0, p, stream);
 }
 
-// How a call is laid out: CTAs of a sequence's own part, by what most have (where there is more a CTA's run is longer): 256 tokens each, more where that makes over 14 CTAs per SM; and whether
+// How a call is laid out: CTAs of a sequence's own part, by what it has room for (where there is more a CTA's run is longer): 256 tokens each, more where that makes over 14 CTAs per SM; and whether
 // four warps join a head.  Heads with many pieces are summed by four: 13 sequences with 37 pieces of 32k tokens 35 -> 31 us; with 5 or fewer one warp does (64 sequences 55 against 57).
 static std::tuple<int64_t, bool> split_of(int64_t B, int64_t hq, int64_t hkv, int64_t pieces, int64_t room) {
   const int64_t wide = B * hkv * ((hq / hkv + ow::HEADS - 1) / ow::HEADS);
@@ -713,7 +713,7 @@ std::tuple<int64_t, bool> paged_shared_split(int64_t sequences, int64_t heads, i
   return split_of(sequences, heads, kv_heads, pieces, room);
 }
 
-// One query token per sequence; pieces: slots of a sequence at most; room: tokens that most sequences have at most beside their prefix (what their split is chosen by); plan int32
+// One query token per sequence; pieces: slots of a sequence at most; room: tokens that a sequence has at most beside its prefix (what their split is chosen by); plan int32
 // [items · 8 + B · 4]: the items, then for every sequence the tokens of its prefix, its first slot, its slots and its row in them.
 torch::Tensor paged_attn_shared(const torch::Tensor& q, const torch::Tensor& kc, const torch::Tensor& vc, const torch::Tensor& tables, const torch::Tensor& seq_lens, const torch::Tensor& plan,
                                 int64_t items, int64_t slots, int64_t pieces, int64_t room, double scale) {

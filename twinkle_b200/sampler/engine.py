@@ -270,10 +270,11 @@ class NativeEngine:
             own = [s.length - b * bs for s, b in zip(seqs, (b for n, b in zip(sizes, blocks) for _ in range(n)))]
             if not self.share_from or self._pays(sizes, blocks, own, bs << max(max(len(s.blocks) for s in seqs) - 1, 0).bit_length()):
                 sizes, blocks = sizes + [1] * (rows - len(seqs)), blocks + [0] * (rows - len(seqs))
-                plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device)
+                most = max(len(s.blocks) - b for s, b in zip(seqs, (b for n, b in zip(sizes, blocks) for _ in range(n)))) * bs
+                plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device, own=most)
                 if captured:      # room in steps, so that the plans of a shrinking batch take the same graphs; a call's workspace goes by it
                     room = min(ops.prefix_items(rows, kv_heads, self.device, heads // kv_heads), max(16, 1 << (plan.items - 1).bit_length()))
-                    plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device, room)
+                    plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device, room, most)
             self._plan = key, plan
         return self._plan[1]
 
@@ -475,8 +476,6 @@ class NativeEngine:
             Bb = 1 << max(B - 1, 0).bit_length()
             Mb = 1 << max(max_blocks - 1, 0).bit_length()
             prefix = self._shared(seqs, Bb, captured=True) if self._share_captured else None
-            if prefix is not None:
-                prefix = prefix._replace(own=max(max_blocks - prefix.shared, 0) * self.cache.block_size)
             st = self._captured(Bb, Mb, prefix)
             if st is None and prefix is not None:       # pages are then read per sequence
                 self._share_captured, prefix = False, None
