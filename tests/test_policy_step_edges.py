@@ -137,3 +137,12 @@ def test_own_pages_are_cut_by_the_longest_own_part():
     for s in seqs[:3]:
         s.origin = seqs[0]
     assert eng._shared(seqs, 5).own == 8 * (50 + 60) and eng._shared(seqs[:3], 3).own == 8 * 12
+
+
+def test_a_plan_is_made_again_when_answers_have_other_room():
+    eng, seqs = _engine_and('tiny-dense', 3, num_blocks=2000, block_size=8)
+    eng.share_from = 0
+    for room in (12, 80):
+        for s in seqs:
+            s.prompt, s.blocks, s.origin = [1] * 800, [1] * (100 + room), seqs[0]
+        assert eng._shared(seqs, 3).own == 8 * room

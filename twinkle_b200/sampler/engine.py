@@ -264,11 +264,13 @@ class NativeEngine:
         heads, kv_heads = self._heads()
         if not any(blocks):
             return None
-        key = (tuple(sizes), tuple(blocks), rows, captured, self.share_from, seqs[0].length >> 8)      # which way is faster changes with the answers' lengths, but slowly
+        # which way is faster changes with the answers' lengths, but slowly; and with the room that they have
+        widest, longest = max(len(s.blocks) for s in seqs), max(s.length for s in seqs)
+        key = (tuple(sizes), tuple(blocks), rows, captured, self.share_from, widest, longest >> 8)
         if self._plan[0] != key:
             bs, plan = self.cache.block_size, None
             own = [s.length - b * bs for s, b in zip(seqs, (b for n, b in zip(sizes, blocks) for _ in range(n)))]
-            if not self.share_from or self._pays(sizes, blocks, own, bs << max(max(len(s.blocks) for s in seqs) - 1, 0).bit_length()):
+            if not self.share_from or self._pays(sizes, blocks, own, bs << max(widest - 1, 0).bit_length()):
                 sizes, blocks = sizes + [1] * (rows - len(seqs)), blocks + [0] * (rows - len(seqs))
                 most = max(len(s.blocks) - b for s, b in zip(seqs, (b for n, b in zip(sizes, blocks) for _ in range(n)))) * bs
                 plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device, own=most)
