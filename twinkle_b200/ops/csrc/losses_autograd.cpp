@@ -18,31 +18,37 @@ torch::Tensor preference_loss_bwd(const torch::Tensor&, const torch::Tensor&, co
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
-// The inputs of a call with the versions that they had: the plain form would otherwise differentiate another call.
-static void keep(AutogradContext* ctx, bool twice, const std::vector<OptT>& inputs) {
-  if (!twice) return;
+// A call as it was made: its inputs with the versions that they had (the plain form would otherwise differentiate another call), the numbers of its rules, and its other numbers.  One entry:
+// each costs a us.
+static void keep(AutogradContext* ctx, const std::vector<OptT>& inputs, std::vector<int64_t> rules, std::vector<double> numbers) {
   std::vector<at::Tensor> tensors;
   std::vector<int64_t> versions;
   for (const auto& t : inputs) {
     tensors.push_back(t.has_value() ? *t : at::Tensor());
     versions.push_back(t.has_value() && t->defined() && !t->is_inference() ? t->_version() : 0);
   }
-  ctx->saved_data["inputs"] = tensors;
-  ctx->saved_data["versions"] = versions;
+  ctx->saved_data["call"] = c10::ivalue::Tuple::create(std::move(tensors), std::move(versions), std::move(rules), std::move(numbers));
 }
+struct Call {
+  std::vector<at::Tensor> inputs;
+  std::vector<int64_t> rules;
+  std::vector<double> numbers;
+};
 // Whether a backward pass wants what the kernels do not give
 static bool plain_wanted(AutogradContext* ctx, const torch::Tensor& g) {
   const bool more = at::GradMode::is_enabled() || !g.has_storage();      // without storage: a wrapper of several
-  TORCH_CHECK(!more || ctx->saved_data.count("inputs") != 0, "the loss kernels have no second derivative, and take one gradient of the loss");
+  TORCH_CHECK(!more || ctx->saved_data.count("call") != 0, "the loss kernels have no second derivative, and take one gradient of the loss");
   return more;
 }
-static std::vector<at::Tensor> kept(AutogradContext* ctx) {
-  auto tensors = ctx->saved_data["inputs"].toTensorVector();
-  const auto versions = ctx->saved_data["versions"].toIntVector();
-  for (size_t i = 0; i < tensors.size(); ++i)
-    TORCH_CHECK(!tensors[i].defined() || tensors[i].is_inference() || tensors[i]._version() == versions[i],
+static Call kept(AutogradContext* ctx) {
+  const auto call = ctx->saved_data["call"].toTuple();
+  const auto& parts = call->elements();
+  const auto versions = parts[1].toIntVector();
+  Call c{parts[0].toTensorVector(), parts[2].toIntVector(), parts[3].toDoubleVector()};
+  for (size_t i = 0; i < c.inputs.size(); ++i)
+    TORCH_CHECK(!c.inputs[i].defined() || c.inputs[i].is_inference() || c.inputs[i]._version() == versions[i],
                 "an input of a loss was modified by an inplace operation before its gradient was differentiated");
-  return tensors;
+  return c;
 }
 // Gradients by the plain form: `form` of ops/reference.py with its arguments and the tensors that want one.  Errors come as C++ exceptions: the engine keeps them in threads without Python.
 template <typename... A>
@@ -66,33 +72,32 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logps, const OptT& ent, const torch::Tensor& labels, const torch::Tensor& adv, const OptT& old, const OptT& ref,
                                int64_t ratio, int64_t kind, int64_t reduce, double eps_low, double eps_high, double beta, double entropy, double tau_pos, double tau_neg, double denominator,
                                int64_t ignore, bool twice) {
-    keep(ctx, twice, {logps, ent, labels, adv, old, ref});
-    ctx->saved_data["rules"] = std::vector<int64_t>{ratio, kind, reduce};
-    ctx->saved_data["numbers"] = std::vector<double>{eps_low, eps_high, beta, entropy, tau_pos, tau_neg, denominator};
+    if (twice) keep(ctx, {logps, ent, labels, adv, old, ref}, {ratio, kind, reduce}, {eps_low, eps_high, beta, entropy, tau_pos, tau_neg, denominator});
     at::AutoDispatchBelowADInplaceOrView below;
     auto out = policy_loss_fwd(logps, labels, adv, old, ref, ent, ratio, kind, reduce, eps_low, eps_high, beta, entropy, tau_pos, tau_neg, denominator, ignore, logps.requires_grad());
     ctx->save_for_backward({out[2], out[3], labels});
+    ctx->saved_data["entropy"] = entropy;
     ctx->saved_data["ignore"] = ignore;
     ctx->mark_non_differentiable({out[1]});
     return {out[0], out[1]};
   }
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     const bool by_logps = ctx->needs_input_grad(0), by_ent = ctx->needs_input_grad(1);
-    const auto numbers = ctx->saved_data["numbers"].toDoubleVector();
     const int64_t ignore = ctx->saved_data["ignore"].toInt();
     variable_list grads(18);
     if (plain_wanted(ctx, g[0])) {
-      const auto x = kept(ctx);       // log-probs, entropies, labels, advantages, old, reference
+      const auto call = kept(ctx);
+      const auto& x = call.inputs;       // log-probs, entropies, labels, advantages, old, reference
       std::vector<at::Tensor> wanted;
       if (by_logps) wanted.push_back(x[0]);
       if (by_ent) wanted.push_back(x[1]);
-      const auto out = plain_gradient("policy_loss_gradient", g[0], wanted, x[0], x[2], x[3], given(x[4]), given(x[5]), given(x[1]), ctx->saved_data["rules"].toIntVector(), numbers, ignore);
+      const auto out = plain_gradient("policy_loss_gradient", g[0], wanted, x[0], x[2], x[3], given(x[4]), given(x[5]), given(x[1]), call.rules, call.numbers, ignore);
       if (by_logps) grads[0] = out[0];
       if (by_ent) grads[1] = out[by_logps ? 1 : 0];
       return grads;
     }
     const auto saved = ctx->get_saved_variables();
-    auto out = policy_loss_bwd(scalar_grad(g[0]), by_logps ? OptT(saved[0]) : OptT(), saved[1], saved[2], numbers[3], ignore, by_ent);
+    auto out = policy_loss_bwd(scalar_grad(g[0]), by_logps ? OptT(saved[0]) : OptT(), saved[1], saved[2], ctx->saved_data["entropy"].toDouble(), ignore, by_ent);
     if (by_logps) grads[0] = out[0];
     if (by_ent) grads[1] = out[1];
     return grads;
@@ -102,9 +107,7 @@ struct PolicyLoss : torch::autograd::Function<PolicyLoss> {
 struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   static variable_list forward(AutogradContext* ctx, const torch::Tensor& logps, const torch::Tensor& labels, const OptT& ref, int64_t form, double beta, double gamma, double smoothing,
                                double nll, int64_t ignore, bool twice) {
-    keep(ctx, twice, {logps, labels, ref});
-    ctx->saved_data["form"] = form;
-    ctx->saved_data["numbers"] = std::vector<double>{beta, gamma, smoothing, nll};
+    if (twice) keep(ctx, {logps, labels, ref}, {form}, {beta, gamma, smoothing, nll});
     at::AutoDispatchBelowADInplaceOrView below;
     auto out = preference_loss_fwd(logps, labels, ref, form, beta, gamma, smoothing, nll, ignore);
     ctx->save_for_backward({out[2], labels});
@@ -115,9 +118,9 @@ struct PreferenceLoss : torch::autograd::Function<PreferenceLoss> {
   static variable_list backward(AutogradContext* ctx, const variable_list& g) {
     variable_list grads(10);
     if (plain_wanted(ctx, g[0])) {
-      const auto x = kept(ctx);
-      grads[0] = plain_gradient("preference_loss_gradient", g[0], {x[0]}, x[0], x[1], given(x[2]), ctx->saved_data["form"].toInt(), ctx->saved_data["numbers"].toDoubleVector(),
-                                ctx->saved_data["ignore"].toInt())[0];
+      const auto call = kept(ctx);
+      const auto& x = call.inputs;
+      grads[0] = plain_gradient("preference_loss_gradient", g[0], {x[0]}, x[0], x[1], given(x[2]), call.rules[0], call.numbers, ctx->saved_data["ignore"].toInt())[0];
       return grads;
     }
     const auto saved = ctx->get_saved_variables();
