@@ -940,7 +940,7 @@ def paged_attention_shared(q, k_cache, v_cache, block_tables, seq_lens, prefix: 
 def cache_copy(pools, src, dst, tokens=None) -> None:
     """In every pool ``[rows, ...]`` row ``dst[i]`` becomes row ``src[i]``, or with ``tokens`` its first ``tokens[i]`` entries along the second dimension do: pages of a paged
     cache that fork or move, slots of recurrent state.  One launch for all pools and up to 2048 pairs.  The pairs are lists of numbers (they travel with the launch).  A row that is written is neither
-    written nor read by another pair."""
+    written nor read by another pair; pools do not overlap."""
     pools = [p for p in pools if p is not None]
     if not pools:
         return
@@ -1208,7 +1208,7 @@ def preference_loss(logps, labels, ref_logps=None, form: str = 'sigmoid', beta: 
     """``(loss, stats)`` of pairs of rows, chosen ``0::2`` and rejected ``1::2``; differentiable by ``logps [B, S]`` (``twice``: see ``policy_loss``).
 
     A row's level is the sum of its log-probs less that of ``ref_logps`` (``[B, S]``, or ``[B]`` summed already), for ``simpo`` and ``orpo`` their mean per token without a reference.  With
-    ``z = beta (chosen − rejected) − gamma`` a pair costs ``−log σ(z)``, smoothed (``sigmoid``, ``simpo``), ``max(0, 1 − z)`` (``hinge``), ``(z − 1 / (2 beta))²`` (``ipo``), ``1 − σ(beta chosen) + σ(beta rejected)``
+    ``z = beta (chosen − rejected) − gamma`` a pair costs ``−log σ(z)``, smoothed (``sigmoid``, ``simpo``), ``max(0, 1 − z)`` (``hinge``), ``(z − 1 / (2 beta))²`` (``ipo``, as the loss classes have it: the published loss has the margin without ``beta`` in place of ``z``), ``1 − σ(beta chosen) + σ(beta rejected)``
     (``kto_pair``) or ``−beta log σ`` of the log odds ratio (``orpo``); pairs are averaged, and ``nll_weight`` times the chosen rows' negative log-likelihood per chosen token is added.  ``stats``: ``beta`` times the
     mean levels of the chosen and rejected rows and of their difference, share of pairs whose chosen row is above, mean summed log-probs of both."""
     if form not in _PREFERENCE:

@@ -5,13 +5,14 @@
 // loss writes each token's derivative without the row's weight, which is known only when all rows are; its backward pass reads that one number
 // per token.  Paired losses have one derivative per row: their backward pass reads the labels.
 //
-// Measured, us on the device: 64 x 4095 tokens with reference, entropies and advantages per token 6.4 + 2.5 (joining) and 3.6 (backward); sequence ratios of 256 x 16384 27 (84 MB read, 17 written:
-// 3.7 TB/s) and 6.9; 512 x 8192 pairs 14 (67 MB: 4.8 TB/s) and 8.3.  A token's inputs behind a branch on its label made each batch of loads wait for the one before (53 and 28 us); with every
-// thread of a cluster reading the others' sums those reads took longer than the tokens (95 and 40).  On the host a step with its gradient takes 80 us, 50 of them torch's engine.
+// Measured, us on the device: 64 x 4095 tokens with reference, entropies and advantages per token 5.9 + 2.5 (joining) and 3.6 (backward); sequence ratios of 256 x 16384 27 (84 MB read, 17 written:
+// 3.7 TB/s) and 7.1; 512 x 8192 pairs 14 (67 MB: 4.8 TB/s) and 8.4.  A token's inputs behind a branch on its label made each batch of loads wait for the one before (53 and 28 us); with every
+// thread of a cluster reading the others' sums those reads took longer than the tokens (95 and 40).  On the host a step with its gradient takes 85 to 110 us, 50 of them torch's engine.  Exact
+// exponentials and quotients cost nothing here (5.9 and 27 us as with fast ones, whose results were two to three times as far from 64 bits).
 //
 // Precision: per token in fp32, sums over tokens and rows in fp64 (a loss is a small difference of sums of advantages).  Differences of log-probs are formed in fp64 and compared
-// with the logarithms of the bounds, so that a token at a bound falls on the right side; e^d − 1 and e^d − d − 1 of small d come from a series.  Exponentials and quotients are the exact
-// functions', not the fast ones': nothing here is bound by arithmetic.  The file is compiled without fast math.
+// with the logarithms of the bounds, so that a token at a bound falls on the right side; e^d − 1 and e^d − d − 1 of small d come from a series.  The file is compiled
+// without fast math.
 // Masked tokens are not read into any sum: infinities and NaN there have no effect.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>

@@ -1,4 +1,4 @@
-// Autograd of the losses in losses.cu.  A micro-batch's kernels take 12 us, so a step's time is the host's: 115 us through a Function in Python, 80 to 90 here, 50 of which torch's
+// Autograd of the losses in losses.cu.  A micro-batch's kernels take 12 us, so a step's time is the host's: 115 us through a Function in Python, 85 to 110 here, 50 of which torch's
 // engine takes for any gradient.
 //
 // The kernels have a first derivative only, for one gradient of the loss.  A call that asks for more (`twice`) keeps its inputs as they are, and a backward pass that is itself
