@@ -270,7 +270,7 @@ class NativeEngine:
         if self._plan[0] != key:
             bs, plan = self.cache.block_size, None
             own = [s.length - b * bs for s, b in zip(seqs, (b for n, b in zip(sizes, blocks) for _ in range(n)))]
-            if not self.share_from or self._pays(sizes, blocks, own, bs << max(widest - 1, 0).bit_length()):
+            if not self.share_from or self._pays(sizes, blocks, own, bs << max(widest - 1, 0).bit_length(), captured):
                 sizes, blocks = sizes + [1] * (rows - len(seqs)), blocks + [0] * (rows - len(seqs))
                 most = max(len(s.blocks) - b for s, b in zip(seqs, (b for n, b in zip(sizes, blocks) for _ in range(n)))) * bs
                 plan = ops.shared_prefix(sizes, blocks, bs, heads, kv_heads, self.device, own=most)
@@ -280,13 +280,14 @@ class NativeEngine:
             self._plan = key, plan
         return self._plan[1]
 
-    def _pays(self, sizes: Sequence[int], blocks: Sequence[int], own: Sequence[int], room: int) -> bool:
-        """Whether a step of these groups is expected to be faster with shared pages read once; never where the kernel does not take the cache."""
+    def _pays(self, sizes: Sequence[int], blocks: Sequence[int], own: Sequence[int], room: int, captured: bool) -> bool:
+        """Whether a step of these groups is expected to be faster with shared pages read once; never where the kernel does not take the cache.  An eager step, whose time is mostly the
+        host's, has to save the 9 us that the call takes longer there (20 against 11)."""
         (heads, kv_heads), (_, width, value) = self._heads(), self.cfg.kv_layout()[0]
         if self.dtype != torch.bfloat16 or width not in (64, 128) or value != width or self.cache.block_size % 8:
             return False
         together, apart = ops.shared_times(sizes, blocks, own, self.cache.block_size, heads, kv_heads, width, room, self.device)
-        return apart > self.share_from * together
+        return apart > self.share_from * together + (0.0 if captured else 9.0)
 
     def _heads(self) -> Tuple[int, int]:
         return self.cfg.num_attention_heads, self.cfg.kv_layout()[0][0]
