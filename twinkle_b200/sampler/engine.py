@@ -231,6 +231,9 @@ class NativeEngine:
             raise ValueError(f'fork: the state of the sequence has seen {len(origin.tokens)} tokens behind its prompt')
         if self.cache.num_slots and len(seqs) > len(self.cache.free_slots):
             raise RuntimeError(f'per-sequence state exhausted: {len(seqs)} forks, {len(self.cache.free_slots)} slots')
+        self._fork(origin, seqs)
+
+    def _fork(self, origin: _Seq, seqs: Sequence[_Seq]) -> None:
         lists, copies = self.cache.fork(origin.blocks, len(origin.prompt), [self.cache.blocks_for(len(s.prompt) + (s.params.max_tokens or 0) + 1) for s in seqs])
         slots = []
         for s, blocks in zip(seqs, lists):
@@ -599,7 +602,7 @@ class NativeEngine:
         for i in run:
             others = [seqs[j] for j in order if firsts[j] == i and j != i and not seqs[j].params.scoring_only]
             if others:
-                self.fork(seqs[i], others)
+                self._fork(seqs[i], others)
         return [seqs[i] for i in order], hidden, [row[firsts[i]] for i in order]
 
     def _run_group(self, seqs: List[_Seq], responses, eos, on_token) -> None:
