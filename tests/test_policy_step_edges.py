@@ -41,7 +41,7 @@ def _engine_and(stack, n, **args):
     return eng, [_Seq(0, [3, 4, 5, 6, 7, 8], SamplingParams(max_tokens=4)) for _ in range(n)]
 
 
-@pytest.mark.parametrize('what', ['has not run', 'other prompt', 'longer prompt', 'other adapter', 'has run', 'has tokens'])
+@pytest.mark.parametrize('what', ['has not run', 'other prompt', 'longer prompt', 'other adapter', 'has run', 'has tokens', 'twice'])
 def test_forks_that_are_refused(what):
     eng, (a, b, c) = _engine_and('tiny-dense', 3)
     if what != 'has not run':
@@ -58,7 +58,7 @@ def test_forks_that_are_refused(what):
         b.tokens.append(1)
     free, held = list(eng.cache.free), list(b.blocks)
     with pytest.raises(ValueError):
-        eng.fork(a, [c, b])
+        eng.fork(a, [c, b, c] if what == 'twice' else [c, b])
     assert eng.cache.free == free and not eng.cache.sharers and b.blocks == held and c.blocks == [] and a.origin is None
 
 

@@ -225,8 +225,8 @@ class NativeEngine:
     def fork(self, origin: _Seq, seqs: Sequence[_Seq]) -> None:
         """Let ``seqs`` continue the prompt of ``origin``, which has run: its full blocks are shared, the rest and the state are copied (a state that has gone beyond the prompt cannot be)."""
         who = lambda s: (s.prompt, s.slot, s.lora_rank, s.lora_scale, s.lora_target)  # noqa: E731
-        if not origin.blocks or any(who(s) != who(origin) or s.blocks or s.tokens for s in seqs):
-            raise ValueError('fork: a sequence that has run, and others that have not, with its prompt and adapter')
+        if not origin.blocks or len({id(s) for s in seqs}) < len(seqs) or any(who(s) != who(origin) or s.blocks or s.tokens for s in seqs):
+            raise ValueError('fork: a sequence that has run, and others that have not, each once, with its prompt and adapter')
         if origin.tokens and (origin.state_slot or origin.linear):
             raise ValueError(f'fork: the state of the sequence has seen {len(origin.tokens)} tokens behind its prompt')
         if self.cache.num_slots and len(seqs) > len(self.cache.free_slots):
